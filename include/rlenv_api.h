@@ -150,6 +150,61 @@ size_t rl_stem_bwd_work_bytes(void);
 int rl_stem_bwd(const void* grad, const void* obs, const void* emph, const void* pal4, void* dw, void* db,
                 long long batch, int packed, void* work, size_t work_bytes, int* err, void* stream);
 
+// ---------------------------------------------------------------- policy operators (rl/model.py:64-72, 176-194)
+
+// Types of the tensors below: 0 fp32, 1 bf16, 2 fp16. Strides are in values, from one row to the next (0 repeats a row);
+// a row's own values are adjacent. All pointers are device pointers unless said otherwise; asynchronous on `stream`;
+// non-zero on a bad argument or launch error (message: rl_norm_error / rl_heads_error, thread-local).
+
+// Layer norm over rows of `width` values: s = x, or x + residual rounded to x's type and written to sum [rows, width];
+// y [rows, width] = (s - mean) / sqrt(variance + eps) * weight + bias, of x's type or fp32. weight, bias [width] of
+// w_type, each may be NULL (1 and 0). stats: NULL, or fp32 [rows, 2] = mean and 1 / sqrt(variance + eps) of each row
+// for the backward. fp32 arithmetic, every output rounded once.
+int rl_norm_fwd(const void* x, const void* residual, const void* weight, const void* bias, void* y, void* sum, void* stats,
+                long long rows, long long width, long long x_stride, long long r_stride, int x_type, int y_type,
+                int w_type, float eps, void* stream);
+// Its gradients: gy (of y_type), gsum (of x_type, NULL: none) = the gradients of y and sum; s, stats = the rows that were
+// normalised and their statistics -> dx [rows, width] of x_type (the residual's too), dweight, dbias [width] of w_type;
+// each may be NULL. work: device scratch of rl_norm_bwd_work_bytes(rows, width) bytes (partial sums, added in a fixed
+// order: the result is deterministic), needed for dweight or dbias.
+size_t rl_norm_bwd_work_bytes(long long rows, long long width);
+int rl_norm_bwd(const void* gy, const void* gsum, const void* s, const void* stats, const void* weight, void* dx,
+                void* dweight, void* dbias, long long rows, long long width, long long gy_stride, long long gsum_stride,
+                long long s_stride, int x_type, int y_type, int w_type, void* work, size_t work_bytes, void* stream);
+const char* rl_norm_error(void);
+
+// Moves drawn from the policy's ordered heads: logits [rows, 19] (the parts of the mask bytes), cond = host array of ten
+// device pointers (or NULL: the parts do not see each other), cond[k (k-1) / 2 + j] = [choices of part j, choices of
+// part k] added to part k's logits for the earlier part j < k's choice; masks u8 [rows, 19], u fp32 [rows, 5] in [0, 1).
+// temperature (0: the best choice), top_k (0: all), top_p, min_p for all rows, or for each row where its pointer is not
+// NULL (fp32, i32, fp32, fp32 [rows]). ids i16 [rows] packed moves, logp fp32 [rows] their log-probability under the
+// distribution that was drawn from. A part with nothing legal answers 0 and adds nothing. Equal logits rank by index.
+int rl_moves_sample(const void* logits, long long stride, int type, const void* const* cond, int cond_type,
+                    const void* masks, long long mask_stride, const void* u, float temperature, int top_k, float top_p,
+                    float min_p, const void* temperatures, const void* top_ks, const void* top_ps, const void* min_ps,
+                    void* ids, void* logp, long long rows, void* stream);
+// The same for rows of `width` (1 .. 4096) choices: legal u8 [rows, legal_width] with a byte for each choice, or the 19
+// mask bytes where width is 324 (the packed moves), or NULL; u fp32 [rows]; choice i64 [rows], logp fp32 [rows].
+int rl_sample(const void* logits, long long stride, int type, int width, const void* legal, long long legal_stride,
+              int legal_width, const void* u, float temperature, int top_k, float top_p, float min_p,
+              const void* temperatures, const void* top_ks, const void* top_ps, const void* min_ps, void* choice,
+              void* logp, long long rows, void* stream);
+// Log-probability and entropy (the parts' conditional entropies along the move) fp32 [rows] of given moves ids i16 [rows]
+// under the ordered heads, without temperature or truncation. A move that the masks exclude has -inf, an id outside
+// 0 .. 323 NaN in both.
+int rl_moves_logp(const void* logits, long long stride, int type, const void* const* cond, int cond_type,
+                  const void* masks, long long mask_stride, const void* ids, void* logp, void* entropy, long long rows,
+                  void* stream);
+// Its gradients: glp, gent fp32 (strides in values; either may be NULL) -> dlogits [rows, 19] of `type` and dcond
+// fp32 [127], the ten tables' gradients laid end to end; each may be NULL. work: rl_moves_logp_bwd_work_bytes() bytes,
+// needed for dcond (partial sums, added in a fixed order: the result is deterministic).
+size_t rl_moves_logp_bwd_work_bytes(void);
+int rl_moves_logp_bwd(const void* glp, long long glp_stride, const void* gent, long long gent_stride, const void* logits,
+                      long long stride, int type, const void* const* cond, int cond_type, const void* masks,
+                      long long mask_stride, const void* ids, void* dlogits, void* dcond, long long rows, void* work,
+                      size_t work_bytes, void* stream);
+const char* rl_heads_error(void);
+
 // No reference counterpart (the reference sums its rollout statistics in Python from the rollout buffers,
 // rl/train.py:450): acc = device float64[4] to which every later decision adds the finished episodes' count, their
 // deaths, their returns and the level events (added by the finishing kernel, no extra launch; the order of the fp64

@@ -9,14 +9,19 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 #include "../../include/rlenv_api.h"   // rl_norm_* compiled against their C-ABI declarations
 
 namespace {
 
-constexpr int kWideThreads = 256;
-constexpr int kColThreads = 256, kCols = 64, kColRows = kColThreads / kCols;
+constexpr int kThreads = 256;
+constexpr int kDevices = 64;                               // whose properties are kept
+constexpr int kMaxRow = 8192;                              // values of a row that a block's registers hold
+constexpr int kCols = 64, kColRows = kThreads / kCols;
+constexpr int kFwdWarps = 16, kBwdWarps = 16;              // warps per SM that share the rows
 
 thread_local std::string g_norm_error;
 
@@ -65,41 +70,389 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// The sum of v over the block's threads, in every thread.
-__device__ __forceinline__ float block_sum(float v, float* red) {
-    v = warp_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float t = 0.f;
-    for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) t += red[w];
-    return t;
+// ------------------------------------------------------------------ rows that fit registers (width <= 8192)
+//
+// TPR threads share a row, EPT values each, in vectors of 16 bytes (VEC) or one by one: vector v of thread t starts at
+// value (v TPR + t) VE. A block of 256 threads (512 for the widest rows) takes 256 / TPR rows at a time and goes on to the
+// next ones, whose values are on their way to shared memory meanwhile; the weights stay in registers. Rows that are not
+// 16-byte aligned are read one value at a time, as they are needed.
+
+template <class TX, bool VEC, int TPR, int EPT>
+struct Tile {
+    static constexpr int kVe = VEC ? 16 / static_cast<int>(sizeof(TX)) : 1;   // values of a vector
+    static constexpr int kNv = EPT / kVe;                                     // vectors of a thread
+    static constexpr int kBlock = TPR > kThreads ? TPR : kThreads;
+    static constexpr int kRows = kBlock / TPR;                                // rows of a block
+    static_assert(kNv * kVe == EPT && kRows * TPR == kBlock, "whole vectors, whole rows");
+    __device__ static int at(int v, int t) { return (v * TPR + t) * kVe; }
+};
+
+template <class T, int N>
+struct alignas(N * sizeof(T) >= 16 ? 16 : N * sizeof(T)) Pack {
+    T v[N];
+};
+
+template <class T, int N>
+__device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
+    return *reinterpret_cast<const Pack<T, N>*>(p);
+}
+template <class T, int N>
+__device__ __forceinline__ void store_pack(T* p, const float* v) {
+    Pack<T, N> q;
+#pragma unroll
+    for (int i = 0; i < N; ++i) q.v[i] = from_f<T>(v[i]);
+    *reinterpret_cast<Pack<T, N>*>(p) = q;
 }
 
-// A row per block at a time, any width; the row is read again (from L1 or L2) for each pass.
+// The sums of two values over a row's TPR threads, in each of them. `red` has two places for each warp of the block and is
+// free again at the next but one call: the calls alternate between its two halves.
+template <int TPR>
+__device__ __forceinline__ float2 row_sums(float x, float y, float2* red) {
+    x = warp_sum(x);
+    y = warp_sum(y);
+    if constexpr (TPR > 32) {
+        const int warp = threadIdx.x >> 5, first = warp & ~(TPR / 32 - 1);
+        if ((threadIdx.x & 31) == 0) red[warp] = make_float2(x, y);
+        __syncthreads();
+        x = y = 0.f;
+#pragma unroll
+        for (int w = 0; w < TPR / 32; ++w) {
+            x += red[first + w].x;
+            y += red[first + w].y;
+        }
+    }
+    return make_float2(x, y);
+}
+
+template <int TPR>
+__device__ __forceinline__ float row_sum(float x, float* red) {
+    x = warp_sum(x);
+    if constexpr (TPR > 32) {
+        const int warp = threadIdx.x >> 5, first = warp & ~(TPR / 32 - 1);
+        if ((threadIdx.x & 31) == 0) red[warp] = x;
+        __syncthreads();
+        x = 0.f;
+#pragma unroll
+        for (int w = 0; w < TPR / 32; ++w) x += red[first + w];
+    }
+    return x;
+}
+
+// A thread's own values of coming rows in shared memory, S rows deep: each thread copies (cp.async, 16 bytes at a time)
+// and reads back only its own slots, so the copies need no barrier and no registers. A slot of N vectors per row lies
+// `kBlock` threads apart: neighbours' 16-byte accesses touch neighbouring banks.
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <class T, int N, int BLOCK>
+__device__ __forceinline__ void copy_pack(uint4* slot, const T* p) {
+    constexpr int kWords = static_cast<int>(sizeof(Pack<T, N>) / 16);
+#pragma unroll
+    for (int q = 0; q < kWords; ++q) copy16(slot + q * BLOCK, reinterpret_cast<const uint4*>(p) + q);
+}
+template <class T, int N, int BLOCK>
+__device__ __forceinline__ Pack<T, N> slot_pack(const uint4* slot) {
+    constexpr int kWords = static_cast<int>(sizeof(Pack<T, N>) / 16);
+    union { Pack<T, N> p; uint4 u[kWords]; } q;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) q.u[i] = slot[i * BLOCK];
+    return q.p;
+}
+
+// Words of 16 bytes that a thread keeps per row of a tensor of T (0: rows are read as they are needed).
+template <class T, bool VEC, int EPT>
+constexpr int kWords = VEC ? EPT * static_cast<int>(sizeof(T)) / 16 : 0;
+// How many rows ahead fit beside `warps` warps per SM in 208 KB, at most 4 (measured: deeper gains nothing).
+template <int WORDS>
+constexpr int depth_of(int warps) {
+    return WORDS == 0 ? 1 : 208 * 1024 / (warps * 32 * 16 * WORDS) < 4 ? 208 * 1024 / (warps * 32 * 16 * WORDS) : 4;
+}
+
+template <class TX, class TY, bool VEC, int TPR, int EPT>
+struct Fwd : Tile<TX, VEC, TPR, EPT> {
+    static constexpr int kW = kWords<TX, VEC, EPT>;
+    static constexpr int kDepth = depth_of<2 * kW>(kFwdWarps);
+    static constexpr size_t kSmem = static_cast<size_t>(kDepth) * 2 * kW * 16 * Fwd::kBlock;
+};
+
+template <class TX, class TY, bool VEC, int TPR, int EPT>
+struct Bwd : Tile<TX, VEC, TPR, EPT> {
+    static constexpr int kW = kWords<TX, VEC, EPT>, kG = kWords<TY, VEC, EPT>;
+    static constexpr int kDepth = depth_of<2 * kW + kG>(kBwdWarps);
+    static constexpr size_t kRing = static_cast<size_t>(kDepth) * (2 * kW + kG) * 16 * Bwd::kBlock;
+    static constexpr size_t kCols = 2 * sizeof(float) * TPR * EPT;   // at the end, in the ring's place
+    static constexpr size_t kSmem = kRing > kCols ? kRing : kCols;
+};
+
+template <class TX, class TY, bool VEC, int TPR, int EPT>
+__global__ void __launch_bounds__(Fwd<TX, TY, VEC, TPR, EPT>::kBlock, kFwdWarps * 32 / Fwd<TX, TY, VEC, TPR, EPT>::kBlock)
+k_norm_fwd(FwdArgs a) {
+    using L = Fwd<TX, TY, VEC, TPR, EPT>;
+    using P = Pack<TX, L::kVe>;
+    constexpr int B = L::kBlock, S = L::kDepth, W = L::kW, E = L::kVe;
+    extern __shared__ uint4 ring[];   // [S][x, residual][W][B]
+    __shared__ float red[2][B / 32];
+    const int t = threadIdx.x % TPR, width = static_cast<int>(a.width);
+    const float inv = 1.f / static_cast<float>(width);
+    float w[EPT], b[EPT];
+#pragma unroll
+    for (int v = 0; v < L::kNv; ++v)
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int c = L::at(v, t) + i;
+            w[v * E + i] = a.weight && c < width ? load_param(a.weight, a.w_type, c) : 1.f;
+            b[v * E + i] = a.bias && c < width ? load_param(a.bias, a.w_type, c) : 0.f;
+        }
+    const long long step = static_cast<long long>(gridDim.x) * L::kRows;
+    long long base = static_cast<long long>(blockIdx.x) * L::kRows;
+    auto fetch = [&](long long row, int slot) {   // one group of copies, empty behind the last row
+        if constexpr (VEC) {
+            if (row < a.rows) {
+                const TX* px = static_cast<const TX*>(a.x) + row * a.x_stride;
+                const TX* pr = static_cast<const TX*>(a.res) + row * a.r_stride;
+                uint4* at = ring + slot * 2 * W * B + threadIdx.x;
+#pragma unroll
+                for (int v = 0; v < L::kNv; ++v)
+                    if (L::at(v, t) < width) {
+                        copy_pack<TX, E, B>(at + v * (W / L::kNv) * B, px + L::at(v, t));
+                        if (a.res) copy_pack<TX, E, B>(at + (W + v * (W / L::kNv)) * B, pr + L::at(v, t));
+                    }
+            }
+            copies_commit();
+        }
+    };
+#pragma unroll
+    for (int q = 0; q < S; ++q) fetch(base + threadIdx.x / TPR + q * step, q);
+    for (int slot = 0; base < a.rows; base += step) {   // the same number of turns for all threads of a block
+        const long long row = base + threadIdx.x / TPR;
+        const bool live = row < a.rows;
+        const TX* px = static_cast<const TX*>(a.x) + row * a.x_stride;
+        const TX* pr = static_cast<const TX*>(a.res) + row * a.r_stride;
+        const uint4* at = ring + slot * 2 * W * B + threadIdx.x;
+        if constexpr (VEC) copies_wait<S - 1>();
+        float s[EPT];
+        float sum = 0.f;
+#pragma unroll
+        for (int v = 0; v < L::kNv; ++v) {
+            const bool in = live && L::at(v, t) < width;
+            P x, r;
+            if (in) {
+                if constexpr (VEC) {
+                    x = slot_pack<TX, E, B>(at + v * (W / L::kNv) * B);
+                    if (a.res) r = slot_pack<TX, E, B>(at + (W + v * (W / L::kNv)) * B);
+                } else {
+                    x = load_pack<TX, E>(px + L::at(v, t));
+                    if (a.res) r = load_pack<TX, E>(pr + L::at(v, t));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                float q = in ? to_f(x.v[i]) : 0.f;
+                if (a.res) q = in ? to_f(from_f<TX>(q + to_f(r.v[i]))) : 0.f;
+                s[v * E + i] = q;
+                sum += q;
+            }
+        }
+        if constexpr (VEC) {
+            fetch(row + S * step, slot);
+            slot = slot + 1 == S ? 0 : slot + 1;
+        }
+        if (a.res && live) {
+            TX* ps = static_cast<TX*>(a.sum) + row * width;
+#pragma unroll
+            for (int v = 0; v < L::kNv; ++v)
+                if (L::at(v, t) < width) store_pack<TX, E>(ps + L::at(v, t), s + v * E);
+        }
+        const float mu = row_sum<TPR>(sum, red[0]) * inv;
+        float sq = 0.f;
+#pragma unroll
+        for (int v = 0; v < L::kNv; ++v)
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                float& q = s[v * E + i];
+                q = L::at(v, t) < width ? q - mu : 0.f;
+                sq = fmaf(q, q, sq);
+            }
+        const float rs = rsqrtf(fmaf(row_sum<TPR>(sq, red[1]), inv, a.eps));
+        if (!live) continue;
+        TY* py = static_cast<TY*>(a.y) + row * width;
+#pragma unroll
+        for (int v = 0; v < L::kNv; ++v)
+            if (L::at(v, t) < width) {
+                float y[E];
+#pragma unroll
+                for (int i = 0; i < E; ++i) y[i] = fmaf(s[v * E + i] * rs, w[v * E + i], b[v * E + i]);
+                store_pack<TY, E>(py + L::at(v, t), y);
+            }
+        if (a.stats && t == 0) a.stats[row] = make_float2(mu, rs);
+    }
+}
+
+// Both gradients in one pass over gy and s: each thread also sums its columns' gy xh and gy over the rows that it sees, and
+// the block writes their sums once, a.splits blocks in all. The row's values are taken from shared memory a second time
+// when their means are known, not kept in registers.
+template <class TX, class TY, bool VEC, int TPR, int EPT>
+__global__ void __launch_bounds__(Bwd<TX, TY, VEC, TPR, EPT>::kBlock, kBwdWarps * 32 / Bwd<TX, TY, VEC, TPR, EPT>::kBlock)
+k_norm_bwd(BwdArgs a) {
+    using L = Bwd<TX, TY, VEC, TPR, EPT>;
+    using PX = Pack<TX, L::kVe>;
+    using PY = Pack<TY, L::kVe>;
+    constexpr int B = L::kBlock, S = L::kDepth, W = L::kW, G = L::kG, E = L::kVe, R = 2 * W + G;
+    extern __shared__ uint4 ring[];   // [S][s, gsum, gy][W, W, G][B]
+    __shared__ float2 red[2][B / 32];
+    int half = 0;
+    const int t = threadIdx.x % TPR, width = static_cast<int>(a.width);
+    const float inv = 1.f / static_cast<float>(width);
+    float w[EPT], dw[EPT], db[EPT];
+#pragma unroll
+    for (int v = 0; v < L::kNv; ++v)
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int c = L::at(v, t) + i;
+            w[v * E + i] = a.weight && c < width ? load_param(a.weight, a.w_type, c) : 1.f;
+            dw[v * E + i] = db[v * E + i] = 0.f;
+        }
+    const long long step = static_cast<long long>(gridDim.x) * L::kRows;
+    long long base = static_cast<long long>(blockIdx.x) * L::kRows;
+    auto fetch = [&](long long row, int slot) {
+        if constexpr (VEC) {
+            if (row < a.rows) {
+                const TX* ps = static_cast<const TX*>(a.s) + row * a.s_stride;
+                const TX* pq = static_cast<const TX*>(a.gsum) + row * a.gsum_stride;
+                const TY* pg = static_cast<const TY*>(a.gy) + row * a.gy_stride;
+                uint4* at = ring + slot * R * B + threadIdx.x;
+#pragma unroll
+                for (int v = 0; v < L::kNv; ++v)
+                    if (L::at(v, t) < width) {
+                        copy_pack<TX, E, B>(at + v * (W / L::kNv) * B, ps + L::at(v, t));
+                        if (a.gsum) copy_pack<TX, E, B>(at + (W + v * (W / L::kNv)) * B, pq + L::at(v, t));
+                        copy_pack<TY, E, B>(at + (2 * W + v * (G / L::kNv)) * B, pg + L::at(v, t));
+                    }
+            }
+            copies_commit();
+        }
+    };
+#pragma unroll
+    for (int q = 0; q < S; ++q) fetch(base + threadIdx.x / TPR + q * step, q);
+    float2 st = make_float2(0.f, 0.f);
+    if (base + threadIdx.x / TPR < a.rows) st = a.stats[base + threadIdx.x / TPR];
+    for (int slot = 0; base < a.rows; base += step) {
+        const long long row = base + threadIdx.x / TPR;
+        const bool live = row < a.rows;
+        const TX* ps = static_cast<const TX*>(a.s) + row * a.s_stride;
+        const TX* pq = static_cast<const TX*>(a.gsum) + row * a.gsum_stride;
+        const TY* pg = static_cast<const TY*>(a.gy) + row * a.gy_stride;
+        const uint4* at = ring + slot * R * B + threadIdx.x;
+        auto value_s = [&](int v) -> PX {
+            if constexpr (VEC) return slot_pack<TX, E, B>(at + v * (W / L::kNv) * B);
+            else return load_pack<TX, E>(ps + L::at(v, t));
+        };
+        auto value_q = [&](int v) -> PX {
+            if constexpr (VEC) return slot_pack<TX, E, B>(at + (W + v * (W / L::kNv)) * B);
+            else return load_pack<TX, E>(pq + L::at(v, t));
+        };
+        auto value_g = [&](int v) -> PY {
+            if constexpr (VEC) return slot_pack<TY, E, B>(at + (2 * W + v * (G / L::kNv)) * B);
+            else return load_pack<TY, E>(pg + L::at(v, t));
+        };
+        if constexpr (VEC) copies_wait<S - 1>();
+        const float mu = st.x, rs = st.y;
+        if (row + step < a.rows) st = a.stats[row + step];
+        float th = 0.f, thx = 0.f;
+#pragma unroll
+        for (int v = 0; v < L::kNv; ++v)
+            if (live && L::at(v, t) < width) {
+                const PX s = value_s(v);
+                const PY g = value_g(v);
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    const int e = v * E + i;
+                    const float q = to_f(g.v[i]), xh = (to_f(s.v[i]) - mu) * rs, h = q * w[e];
+                    dw[e] = fmaf(q, xh, dw[e]);
+                    db[e] += q;
+                    th += h;
+                    thx = fmaf(h, xh, thx);
+                }
+            }
+        const float2 sums = row_sums<TPR>(th, thx, red[half ^= 1]);
+        const float mh = sums.x * inv, mhx = sums.y * inv;
+        if (live && a.dx) {
+            TX* pd = static_cast<TX*>(a.dx) + row * width;
+#pragma unroll
+            for (int v = 0; v < L::kNv; ++v)
+                if (L::at(v, t) < width) {
+                    const PX s = value_s(v);
+                    const PY g = value_g(v);
+                    PX q;
+                    if (a.gsum) q = value_q(v);
+                    float d[E];
+#pragma unroll
+                    for (int i = 0; i < E; ++i) {
+                        const float xh = (to_f(s.v[i]) - mu) * rs;
+                        d[i] = fmaf(fmaf(-xh, mhx, to_f(g.v[i]) * w[v * E + i] - mh), rs, a.gsum ? to_f(q.v[i]) : 0.f);
+                    }
+                    store_pack<TX, E>(pd + L::at(v, t), d);
+                }
+        }
+        if constexpr (VEC) {
+            fetch(row + S * step, slot);
+            slot = slot + 1 == S ? 0 : slot + 1;
+        }
+    }
+    if (!a.part) return;
+    // the block's rows side by side: their column sums, in the order of the groups
+    float* cols = reinterpret_cast<float*>(ring);   // [2][TPR * EPT]; no copy is under way any more
+    if constexpr (VEC) copies_wait<0>();
+    __syncthreads();
+    for (int q = 0; q < L::kRows; ++q) {
+        if (static_cast<int>(threadIdx.x) / TPR == q) {
+#pragma unroll
+            for (int v = 0; v < L::kNv; ++v)
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    const int c = L::at(v, t) + i, e = v * E + i;
+                    cols[c] = q ? cols[c] + dw[e] : dw[e];
+                    cols[TPR * EPT + c] = q ? cols[TPR * EPT + c] + db[e] : db[e];
+                }
+        }
+        __syncthreads();
+    }
+    float* part = a.part + static_cast<long long>(blockIdx.x) * 2 * width;
+    for (int c = threadIdx.x; c < width; c += B) {
+        part[c] = cols[c];
+        part[width + c] = cols[TPR * EPT + c];
+    }
+}
+
+// ------------------------------------------------------------------ wider rows: read again for each pass
+
 template <class TX, class TY>
-__global__ void __launch_bounds__(kWideThreads) k_norm_fwd_wide(FwdArgs a) {
-    __shared__ float red[kWideThreads / 32];
+__global__ void __launch_bounds__(kThreads) k_norm_fwd_wide(FwdArgs a) {
+    __shared__ float red[2][kThreads / 32];
     const float inv = 1.f / static_cast<float>(a.width);
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const TX* x = static_cast<const TX*>(a.x) + row * a.x_stride;
         if (a.res) {
             const TX* r = static_cast<const TX*>(a.res) + row * a.r_stride;
             TX* s = static_cast<TX*>(a.sum) + row * a.width;
-            for (long long i = threadIdx.x; i < a.width; i += blockDim.x) s[i] = from_f<TX>(to_f(x[i]) + to_f(r[i]));
+            for (long long i = threadIdx.x; i < a.width; i += kThreads) s[i] = from_f<TX>(to_f(x[i]) + to_f(r[i]));
             x = s;   // each thread reads back only what it wrote itself
         }
         float t = 0.f;
-        for (long long i = threadIdx.x; i < a.width; i += blockDim.x) t += to_f(x[i]);
-        const float mu = block_sum(t, red) * inv;
+        for (long long i = threadIdx.x; i < a.width; i += kThreads) t += to_f(x[i]);
+        const float mu = row_sum<kThreads>(t, red[0]) * inv;
         t = 0.f;
-        for (long long i = threadIdx.x; i < a.width; i += blockDim.x) {
+        for (long long i = threadIdx.x; i < a.width; i += kThreads) {
             const float c = to_f(x[i]) - mu;
             t = fmaf(c, c, t);
         }
-        const float rs = rsqrtf(fmaf(block_sum(t, red), inv, a.eps));
+        const float rs = rsqrtf(fmaf(row_sum<kThreads>(t, red[1]), inv, a.eps));
         TY* y = static_cast<TY*>(a.y) + row * a.width;
-        for (long long i = threadIdx.x; i < a.width; i += blockDim.x) {
+        for (long long i = threadIdx.x; i < a.width; i += kThreads) {
             const float w = a.weight ? load_param(a.weight, a.w_type, i) : 1.f;
             const float b = a.bias ? load_param(a.bias, a.w_type, i) : 0.f;
             y[i] = from_f<TY>(fmaf((to_f(x[i]) - mu) * rs, w, b));
@@ -109,34 +462,35 @@ __global__ void __launch_bounds__(kWideThreads) k_norm_fwd_wide(FwdArgs a) {
 }
 
 template <class TX, class TY>
-__global__ void __launch_bounds__(kWideThreads) k_norm_dx_wide(BwdArgs a) {
-    __shared__ float red[kWideThreads / 32];
+__global__ void __launch_bounds__(kThreads) k_norm_dx_wide(BwdArgs a) {
+    __shared__ float2 red[2][kThreads / 32];
+    int half = 0;
     const float inv = 1.f / static_cast<float>(a.width);
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const TX* s = static_cast<const TX*>(a.s) + row * a.s_stride;
         const TY* g = static_cast<const TY*>(a.gy) + row * a.gy_stride;
         const float2 st = a.stats[row];
         float th = 0.f, thx = 0.f;
-        for (long long i = threadIdx.x; i < a.width; i += blockDim.x) {
+        for (long long i = threadIdx.x; i < a.width; i += kThreads) {
             const float h = to_f(g[i]) * (a.weight ? load_param(a.weight, a.w_type, i) : 1.f);
             th += h;
             thx = fmaf(h, (to_f(s[i]) - st.x) * st.y, thx);
         }
-        const float mh = block_sum(th, red) * inv, mhx = block_sum(thx, red) * inv;
+        const float2 sums = row_sums<kThreads>(th, thx, red[half ^= 1]);
+        const float mh = sums.x * inv, mhx = sums.y * inv;
         TX* dx = static_cast<TX*>(a.dx) + row * a.width;
         const TX* gs = a.gsum ? static_cast<const TX*>(a.gsum) + row * a.gsum_stride : nullptr;
-        for (long long i = threadIdx.x; i < a.width; i += blockDim.x) {
+        for (long long i = threadIdx.x; i < a.width; i += kThreads) {
             const float h = to_f(g[i]) * (a.weight ? load_param(a.weight, a.w_type, i) : 1.f);
             const float xh = (to_f(s[i]) - st.x) * st.y;
-            const float d = (h - mh - xh * mhx) * st.y;
-            dx[i] = from_f<TX>(gs ? d + to_f(gs[i]) : d);
+            dx[i] = from_f<TX>(fmaf(fmaf(-xh, mhx, h - mh), st.y, gs ? to_f(gs[i]) : 0.f));
         }
     }
 }
 
 // Column sums of gy xh and gy over one split of the rows; a block takes 64 columns, 4 rows at a time.
 template <class TX, class TY>
-__global__ void __launch_bounds__(kColThreads) k_norm_dw_wide(BwdArgs a) {
+__global__ void __launch_bounds__(kThreads) k_norm_dw_wide(BwdArgs a) {
     __shared__ float red[2][kColRows][kCols];
     const int c = threadIdx.x % kCols, q = threadIdx.x / kCols;
     const long long col = static_cast<long long>(blockIdx.x) * kCols + c;
@@ -163,40 +517,101 @@ __global__ void __launch_bounds__(kColThreads) k_norm_dw_wide(BwdArgs a) {
     }
 }
 
-// The splits' partial sums in their order: the result does not depend on which block ran when.
-__global__ void __launch_bounds__(256) k_norm_dw_sum(BwdArgs a) {
-    const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-    if (i >= 2 * a.width) return;
+// The partial sums of 32 columns per block, 8 runs of them side by side and then in order: the result does not depend on
+// which block ran when.
+__global__ void __launch_bounds__(kThreads) k_norm_dw_sum(BwdArgs a) {
+    __shared__ float red[kThreads / 32][32];
+    const long long i = static_cast<long long>(blockIdx.x) * 32 + (threadIdx.x & 31);
+    const int q = threadIdx.x >> 5;
     float t = 0.f;
-    for (int p = 0; p < a.splits; ++p) t += a.part[static_cast<long long>(p) * 2 * a.width + i];
-    const long long col = i < a.width ? i : i - a.width;
-    void* out = i < a.width ? a.dweight : a.dbias;
-    if (out) store_param(out, a.w_type, col, t);
+    if (i < 2 * a.width)
+        for (int p = q; p < a.splits; p += kThreads / 32) t += a.part[static_cast<long long>(p) * 2 * a.width + i];
+    red[q][threadIdx.x & 31] = t;
+    __syncthreads();
+    if (q == 0 && i < 2 * a.width) {
+        for (int j = 1; j < kThreads / 32; ++j) t += red[j][threadIdx.x];
+        void* out = i < a.width ? a.dweight : a.dbias;
+        if (out) store_param(out, a.w_type, i < a.width ? i : i - a.width, t);
+    }
 }
 
+int current_device() {
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess ? dev : -1;
+}
+
+// The current device's SM count, asked once per device.
 int sm_count() {
-    int dev = 0, sms = 148;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    static std::atomic<int> known[kDevices];
+    const int dev = current_device();
+    const bool kept = dev >= 0 && dev < kDevices;
+    int sms = kept ? known[dev].load(std::memory_order_relaxed) : 0;
+    if (sms > 0) return sms;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1) return 148;
+    if (kept) known[dev].store(sms, std::memory_order_relaxed);
     return sms;
 }
 
+// Rows that a block takes at a time.
+int block_rows(long long width) { return width <= 512 ? 8 : width <= 1024 ? 4 : width <= 2048 ? 2 : 1; }
+int block_warps(long long width) { return width <= 4096 ? 8 : 16; }
+
+// Partial sums of the parameters' gradients: blocks of k_norm_bwd, or row splits of k_norm_dw_wide.
 int splits_of(long long rows, long long width) {
-    const long long blocks = (width + kCols - 1) / kCols;
-    long long n = (8ll * sm_count() + blocks - 1) / blocks;
-    const long long most = (rows + 16 * kColRows - 1) / (16 * kColRows);
+    long long n, most;
+    if (width <= kMaxRow) {
+        n = static_cast<long long>(kBwdWarps / block_warps(width)) * sm_count();
+        most = (rows + block_rows(width) - 1) / block_rows(width);
+    } else {
+        const long long blocks = (width + kCols - 1) / kCols;
+        n = (8ll * sm_count() + blocks - 1) / blocks;
+        most = (rows + 16 * kColRows - 1) / (16 * kColRows);
+    }
     if (n > most) n = most;
     return static_cast<int>(n < 1 ? 1 : n);
 }
 
-unsigned wide_grid(long long rows) {
-    const long long most = 8ll * sm_count();
-    return static_cast<unsigned>(rows < most ? rows : most);
+unsigned blocks_of(long long groups, int per_sm) {
+    const long long most = static_cast<long long>(per_sm) * sm_count();
+    return static_cast<unsigned>(groups < most ? groups : most);
+}
+
+// Launches a kernel that may need more shared memory than the 48 KB it has unasked (asked for once per device).
+template <auto KERNEL, class A>
+cudaError_t launch(unsigned grid, int block, size_t smem, cudaStream_t stream, const A& a) {
+    static std::atomic<bool> asked[kDevices];
+    if (smem > 48 * 1024) {
+        const int dev = current_device();
+        if (dev < 0 || dev >= kDevices || !asked[dev].load(std::memory_order_acquire)) {
+            const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+            if (e != cudaSuccess) return e;
+            if (dev >= 0 && dev < kDevices) asked[dev].store(true, std::memory_order_release);
+        }
+    }
+    KERNEL<<<grid, static_cast<unsigned>(block), smem, stream>>>(a);
+    return cudaSuccess;
 }
 
 int failed(const char* msg) {
     g_norm_error = msg;
     return 1;
+}
+
+// f of the row's tile (threads per row, values per thread): the smallest that holds it.
+template <class F>
+void with_tile(long long width, F f) {
+    using std::integral_constant;
+    if (width <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+    else if (width <= 512) f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+    else if (width <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
+    else if (width <= 2048) f(integral_constant<int, 128>{}, integral_constant<int, 16>{});
+    else if (width <= 4096) f(integral_constant<int, 256>{}, integral_constant<int, 16>{});
+    else f(integral_constant<int, 512>{}, integral_constant<int, 16>{});
+}
+
+bool aligned(const void* p, long long stride, int type) {
+    const long long e = type == 0 ? 4 : 2;
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * e % 16 == 0;
 }
 
 // f(TX, TY) of the types of x and y: y has x's type or is fp32.
@@ -234,10 +649,25 @@ int rl_norm_fwd(const void* x, const void* residual, const void* weight, const v
     if (!x || !y || (residual && !sum)) return failed("x, y and (with a residual) sum must be given");
     FwdArgs a{x, residual, weight, bias, y, sum, static_cast<float2*>(stats), rows, width, x_stride, r_stride, w_type, eps};
     auto s = static_cast<cudaStream_t>(stream);
+    cudaError_t e = cudaSuccess;
     with_types(x_type, y_type, [&](auto tx, auto ty) {
-        k_norm_fwd_wide<decltype(tx), decltype(ty)><<<wide_grid(rows), kWideThreads, 0, s>>>(a);
+        using TX = decltype(tx);
+        using TY = decltype(ty);
+        if (width > kMaxRow) {
+            k_norm_fwd_wide<TX, TY><<<blocks_of(rows, 8), kThreads, 0, s>>>(a);
+            return;
+        }
+        const bool vec = width * sizeof(TX) % 16 == 0 && aligned(x, x_stride, x_type) && aligned(residual, r_stride, x_type) &&
+                         aligned(y, 0, y_type) && aligned(sum, 0, x_type);
+        const unsigned grid = blocks_of((rows + block_rows(width) - 1) / block_rows(width), kFwdWarps / block_warps(width));
+        with_tile(width, [&](auto tpr, auto ept) {
+            using V = Fwd<TX, TY, true, tpr(), ept()>;
+            using N = Fwd<TX, TY, false, tpr(), ept()>;
+            e = vec ? launch<k_norm_fwd<TX, TY, true, tpr(), ept()>>(grid, V::kBlock, V::kSmem, s, a)
+                    : launch<k_norm_fwd<TX, TY, false, tpr(), ept()>>(grid, N::kBlock, N::kSmem, s, a);
+        });
     });
-    const cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) e = cudaGetLastError();
     return e == cudaSuccess ? 0 : failed(cudaGetErrorString(e));
 }
 
@@ -255,20 +685,35 @@ int rl_norm_bwd(const void* gy, const void* gsum, const void* s, const void* sta
     const bool params = dweight || dbias;
     if (params && (!work || work_bytes < rl_norm_bwd_work_bytes(rows, width)))
         return failed("work space smaller than rl_norm_bwd_work_bytes()");
-    BwdArgs a{gy, gsum, s, weight, static_cast<const float2*>(stats), dx, dweight, dbias, static_cast<float*>(work),
-              rows, width, gy_stride, gsum_stride, s_stride, w_type, params ? splits_of(rows, width) : 0};
+    BwdArgs a{gy, gsum, s, weight, static_cast<const float2*>(stats), dx, dweight, dbias,
+              params ? static_cast<float*>(work) : nullptr, rows, width, gy_stride, gsum_stride, s_stride, w_type,
+              splits_of(rows, width)};
+    if (!dx && !params) return 0;
     auto q = static_cast<cudaStream_t>(stream);
+    cudaError_t e = cudaSuccess;
     with_types(x_type, y_type, [&](auto tx, auto ty) {
         using TX = decltype(tx);
         using TY = decltype(ty);
-        if (dx) k_norm_dx_wide<TX, TY><<<wide_grid(rows), kWideThreads, 0, q>>>(a);
-        if (params) {
-            const dim3 grid(static_cast<unsigned>((width + kCols - 1) / kCols), static_cast<unsigned>(a.splits));
-            k_norm_dw_wide<TX, TY><<<grid, kColThreads, 0, q>>>(a);
+        if (width > kMaxRow) {
+            if (dx) k_norm_dx_wide<TX, TY><<<blocks_of(rows, 8), kThreads, 0, q>>>(a);
+            if (params) {
+                const dim3 grid(static_cast<unsigned>((width + kCols - 1) / kCols), static_cast<unsigned>(a.splits));
+                k_norm_dw_wide<TX, TY><<<grid, kThreads, 0, q>>>(a);
+            }
+            return;
         }
+        const bool vec = width * sizeof(TX) % 16 == 0 && aligned(s, s_stride, x_type) && aligned(gy, gy_stride, y_type) &&
+                         aligned(gsum, gsum_stride, x_type) && aligned(dx, 0, x_type);
+        with_tile(width, [&](auto tpr, auto ept) {
+            using V = Bwd<TX, TY, true, tpr(), ept()>;
+            using N = Bwd<TX, TY, false, tpr(), ept()>;
+            const auto grid = static_cast<unsigned>(a.splits);
+            e = vec ? launch<k_norm_bwd<TX, TY, true, tpr(), ept()>>(grid, V::kBlock, V::kSmem, q, a)
+                    : launch<k_norm_bwd<TX, TY, false, tpr(), ept()>>(grid, N::kBlock, N::kSmem, q, a);
+        });
     });
-    if (params) k_norm_dw_sum<<<static_cast<unsigned>((2 * width + 255) / 256), 256, 0, q>>>(a);
-    const cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess && params) k_norm_dw_sum<<<static_cast<unsigned>((2 * width + 31) / 32), kThreads, 0, q>>>(a);
+    if (e == cudaSuccess) e = cudaGetLastError();
     return e == cudaSuccess ? 0 : failed(cudaGetErrorString(e));
 }
 

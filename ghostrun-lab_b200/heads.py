@@ -17,6 +17,7 @@ distribution drawn from. The same inputs give the same choice on any launch shap
 nothing legal answers 0, the neutral choice, with log-probability and entropy 0 and no gradient."""
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -31,6 +32,15 @@ MOVES, BYTES, MAX_WIDTH = 324, 19, 4096
 _LIB = None
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _Tables = ctypes.c_void_p * len(TABLES)
+_TABLE_AT = [sum(a * b for a, b in TABLES[:t]) for t in range(len(TABLES) + 1)]   # where each table starts, laid end to end
+_CUT = (('temperature', 1.0, torch.float32), ('top_k', 0, torch.int32), ('top_p', 1.0, torch.float32),
+        ('min_p', 0.0, torch.float32))
+_stream = torch._C._cuda_getCurrentRawStream   # the current stream's handle, without an object made for it
+_HERE = contextlib.nullcontext()
+
+
+def _on(dev):
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def _lib(path=None):
@@ -50,11 +60,11 @@ def _lib(path=None):
 
 
 def _adjacent(t):
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
 def _check_logits(what, logits, width=None):
-    if logits.device.type != 'cuda':
+    if not logits.is_cuda:
         raise RuntimeError(f'{what} runs on the GPU only')
     if logits.dim() != 2 or logits.dtype not in _TYPES or (width is not None and logits.shape[1] != width):
         raise RuntimeError(f'{what}: logits must be [B, {width or "V"}] fp32, bf16 or fp16, got {list(logits.shape)} '
@@ -71,69 +81,69 @@ def _check_bytes(what, name, t, rows, widths, dev):
 
 
 def _check_row(what, name, t, shape, dtype, dev):
-    if tuple(t.shape) != shape or t.dtype != dtype or t.device != dev:
+    if t.shape != shape or t.dtype != dtype or t.device != dev:
         raise RuntimeError(f'{what}: {name} must be {list(shape)} {dtype} on {dev}, got {list(t.shape)} {t.dtype} on '
                            f'{t.device}')
     return t.contiguous()
 
 
 def _check_cond(what, cond, dev):
-    """The tables' pointers (None without tables), their type, and the tensors that the pointers are of."""
+    """The tables, each contiguous; () without tables."""
     if cond is None:
-        return None, 0, ()
+        return ()
     cond = [t.contiguous() for t in cond]
-    if len(cond) != len(TABLES) or any(t.shape != s for t, s in zip(cond, TABLES)):
+    if len(cond) != len(TABLES) or any([t.shape != s for t, s in zip(cond, TABLES)]):
         raise RuntimeError(f'{what}: cond must be ten tables of shapes {TABLES}, got {[tuple(t.shape) for t in cond]}')
     dtype = cond[0].dtype
-    if dtype not in _TYPES or any(t.dtype != dtype or t.device != dev for t in cond):
+    if dtype not in _TYPES or any([t.dtype != dtype or t.device != dev for t in cond]):
         raise RuntimeError(f'{what}: the tables of cond must be fp32, bf16 or fp16, all alike, on {dev}')
-    return _Tables(*[t.data_ptr() for t in cond]), _TYPES[dtype], cond
+    return cond
+
+
+def _pointers(cond):
+    """The tables as the library takes them: an array of their pointers and their type."""
+    return (_Tables(*[t.data_ptr() for t in cond]), _TYPES[cond[0].dtype]) if cond else (None, 0)
 
 
 def _check_cut(what, rows, dev, temperature, top_k, top_p, min_p):
-    """The four parameters as rl_sample takes them (numbers, then pointers), and the tensors that the pointers are of."""
-    numbers, pointers, kept = [], [], []
-    for name, v, off, dtype in (('temperature', temperature, 1.0, torch.float32), ('top_k', top_k, 0, torch.int32),
-                                ('top_p', top_p, 1.0, torch.float32), ('min_p', min_p, 0.0, torch.float32)):
-        if torch.is_tensor(v):
+    """The four parameters as the library takes them (numbers, then pointers), and the tensors that the pointers are of."""
+    values = [temperature, top_k, top_p, min_p]
+    pointers, kept = [None] * 4, []
+    for i, v in enumerate(values):
+        if isinstance(v, torch.Tensor):
+            name, off, dtype = _CUT[i]
             if v.dim() != 1 or v.shape[0] != rows or v.device != dev or v.dtype == torch.bool or v.is_complex() \
                     or (name == 'top_k' and v.is_floating_point()):
                 raise RuntimeError(f'{what}: {name} must be a number or [{rows}] on {dev}, got {list(v.shape)} {v.dtype} '
                                    f'on {v.device}')
             v = v.to(dtype).contiguous()
-            numbers.append(off)
-            pointers.append(v.data_ptr())
+            values[i], pointers[i] = off, v.data_ptr()
             kept.append(v)
-        else:
-            numbers.append(v)
-            pointers.append(None)
-    t, k, p, m = numbers
+    t, k, p, m = values
     if not (t >= 0 and p >= 0 and m <= 1 and 0 <= k < 2 ** 31 and int(k) == k):
         raise RuntimeError(f'{what}: temperature and top_p must be 0 or more, top_k a whole number of 0 or more, min_p at most '
                            f'1; got temperature {t}, top_k {k}, top_p {p}, min_p {m}')
     return (t, int(k), p, m, *pointers), kept
 
 
-def _call(lib, what, rc):
-    if rc != 0:
-        raise RuntimeError(f'{what}: {lib.rl_heads_error().decode()}')
+def _call(lib, name, *args):
+    if getattr(lib, name)(*args) != 0:
+        raise RuntimeError(f'{name}: {lib.rl_heads_error().decode()}')
 
 
 def sample_moves(logits, cond, masks, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, lib_path=None):
     """One move for each row, part by part: (packed ids int16 [B], log-probabilities fp32 [B])."""
     logits = _check_logits('sample_moves', logits, BYTES)
     rows, dev = logits.shape[0], logits.device
-    tables, cond_type, kept = _check_cond('sample_moves', cond, dev)
+    cond = _check_cond('sample_moves', cond, dev)
     masks = _check_bytes('sample_moves', 'masks', masks, rows, (BYTES,), dev)
     u = _check_row('sample_moves', 'u', u, (rows, 5), torch.float32, dev)
-    cut, cut_kept = _check_cut('sample_moves', rows, dev, temperature, top_k, top_p, min_p)
+    cut, kept = _check_cut('sample_moves', rows, dev, temperature, top_k, top_p, min_p)
     ids = torch.empty(rows, dtype=torch.int16, device=dev)
     logp = torch.empty(rows, dtype=torch.float32, device=dev)
-    lib = _lib(lib_path)
-    with torch.cuda.device(dev):
-        _call(lib, 'rl_moves_sample', lib.rl_moves_sample(
-            logits.data_ptr(), logits.stride(0), _TYPES[logits.dtype], tables, cond_type, masks.data_ptr(), masks.stride(0),
-            u.data_ptr(), *cut, ids.data_ptr(), logp.data_ptr(), rows, torch.cuda.current_stream(dev).cuda_stream))
+    with _on(dev):
+        _call(_lib(lib_path), 'rl_moves_sample', logits.data_ptr(), logits.stride(0), _TYPES[logits.dtype], *_pointers(cond),
+              masks.data_ptr(), masks.stride(0), u.data_ptr(), *cut, ids.data_ptr(), logp.data_ptr(), rows, _stream(dev.index))
     return ids, logp
 
 
@@ -146,29 +156,59 @@ def sample(logits, u, legal=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
     if legal is not None:
         legal = _check_bytes('sample', 'legal', legal, rows, (width, BYTES) if width == MOVES else (width,), dev)
     u = _check_row('sample', 'u', u, (rows,), torch.float32, dev)
-    cut, cut_kept = _check_cut('sample', rows, dev, temperature, top_k, top_p, min_p)
+    cut, kept = _check_cut('sample', rows, dev, temperature, top_k, top_p, min_p)
     choice = torch.empty(rows, dtype=torch.int64, device=dev)
     logp = torch.empty(rows, dtype=torch.float32, device=dev)
-    lib = _lib(lib_path)
-    with torch.cuda.device(dev):
-        _call(lib, 'rl_sample', lib.rl_sample(
-            logits.data_ptr(), logits.stride(0), _TYPES[logits.dtype], width, None if legal is None else legal.data_ptr(),
-            0 if legal is None else legal.stride(0), 0 if legal is None else legal.shape[1], u.data_ptr(), *cut,
-            choice.data_ptr(), logp.data_ptr(), rows, torch.cuda.current_stream(dev).cuda_stream))
+    with _on(dev):
+        _call(_lib(lib_path), 'rl_sample', logits.data_ptr(), logits.stride(0), _TYPES[logits.dtype], width,
+              None if legal is None else legal.data_ptr(), 0 if legal is None else legal.stride(0),
+              0 if legal is None else legal.shape[1], u.data_ptr(), *cut, choice.data_ptr(), logp.data_ptr(), rows,
+              _stream(dev.index))
     return choice, logp
 
 
 def _logp_forward(logits, cond, masks, ids, lib_path):
     rows, dev = logits.shape[0], logits.device
-    tables, cond_type, kept = _check_cond('moves_logp', cond, dev)
     logp = torch.empty(rows, dtype=torch.float32, device=dev)
     entropy = torch.empty(rows, dtype=torch.float32, device=dev)
-    lib = _lib(lib_path)
-    with torch.cuda.device(dev):
-        _call(lib, 'rl_moves_logp', lib.rl_moves_logp(
-            logits.data_ptr(), logits.stride(0), _TYPES[logits.dtype], tables, cond_type, masks.data_ptr(), masks.stride(0),
-            ids.data_ptr(), logp.data_ptr(), entropy.data_ptr(), rows, torch.cuda.current_stream(dev).cuda_stream))
+    with _on(dev):
+        _call(_lib(lib_path), 'rl_moves_logp', logits.data_ptr(), logits.stride(0), _TYPES[logits.dtype], *_pointers(cond),
+              masks.data_ptr(), masks.stride(0), ids.data_ptr(), logp.data_ptr(), entropy.data_ptr(), rows,
+              _stream(dev.index))
     return logp, entropy
+
+
+def _logp_gradients(ctx, glp, gent):
+    logits, masks, ids, *cond = ctx.saved_tensors
+    rows, dev, need = logits.shape[0], logits.device, ctx.needs_input_grad
+    dlogits = dcond = work = None
+    if need[0]:
+        dlogits = torch.empty((rows, BYTES), dtype=logits.dtype, device=dev)
+    if any(need[4:]):
+        dcond = torch.empty(_TABLE_AT[-1], dtype=torch.float32, device=dev)
+    if rows == 0 or (glp is None and gent is None):
+        for t in (dlogits, dcond):
+            if t is not None:
+                t.zero_()
+    else:
+        lib = _lib(ctx.lib_path)
+        with _on(dev):
+            nbytes = 0
+            if dcond is not None:
+                nbytes = lib.rl_moves_logp_bwd_work_bytes()
+                work = torch.empty(nbytes // 4, dtype=torch.float32, device=dev)
+            _call(lib, 'rl_moves_logp_bwd', None if glp is None else glp.data_ptr(), 0 if glp is None else glp.stride(0),
+                  None if gent is None else gent.data_ptr(), 0 if gent is None else gent.stride(0), logits.data_ptr(),
+                  logits.stride(0), _TYPES[logits.dtype], *_pointers(cond), masks.data_ptr(), masks.stride(0),
+                  ids.data_ptr(), None if dlogits is None else dlogits.data_ptr(),
+                  None if dcond is None else dcond.data_ptr(), rows, None if work is None else work.data_ptr(), nbytes,
+                  _stream(dev.index))
+    if dcond is None:
+        return (dlogits, None, None, None, *[None] * len(cond))
+    if cond[0].dtype != torch.float32:
+        dcond = dcond.to(cond[0].dtype)
+    tables = [dcond.as_strided(s, (s[1], 1), at) if n else None for s, at, n in zip(TABLES, _TABLE_AT, need[4:])]
+    return (dlogits, None, None, None, *tables)
 
 
 class _MovesLogp(torch.autograd.Function):
@@ -177,38 +217,13 @@ class _MovesLogp(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, masks, ids, *cond)
         ctx.lib_path = lib_path
-        return _logp_forward(logits, cond or None, masks, ids, lib_path)
+        return _logp_forward(logits, cond, masks, ids, lib_path)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, glp, gent):
-        logits, masks, ids, *cond = ctx.saved_tensors
-        rows, dev = logits.shape[0], logits.device
-        want_cond = any(ctx.needs_input_grad[4:])
-        dlogits = torch.empty((rows, BYTES), dtype=logits.dtype, device=dev) if ctx.needs_input_grad[0] else None
-        none = (glp is None and gent is None) or rows == 0
-        dcond = (torch.zeros if none else torch.empty)(sum(a * b for a, b in TABLES), dtype=torch.float32,
-                                                       device=dev) if want_cond else None
-        if none:
-            dlogits = None if dlogits is None else dlogits.zero_()
-        else:
-            tables, cond_type, kept = _check_cond('moves_logp', cond or None, dev)
-            lib = _lib(ctx.lib_path)
-            with torch.cuda.device(dev):
-                nbytes = int(lib.rl_moves_logp_bwd_work_bytes()) if want_cond else 0
-                work = torch.empty(nbytes // 4, dtype=torch.float32, device=dev) if nbytes else None
-                _call(lib, 'rl_moves_logp_bwd', lib.rl_moves_logp_bwd(
-                    None if glp is None else glp.data_ptr(), 0 if glp is None else glp.stride(0),
-                    None if gent is None else gent.data_ptr(), 0 if gent is None else gent.stride(0),
-                    logits.data_ptr(), logits.stride(0), _TYPES[logits.dtype], tables, cond_type, masks.data_ptr(),
-                    masks.stride(0), ids.data_ptr(), None if dlogits is None else dlogits.data_ptr(),
-                    None if dcond is None else dcond.data_ptr(), rows, None if work is None else work.data_ptr(), nbytes,
-                    torch.cuda.current_stream(dev).cuda_stream))
-        grads, at = [], 0
-        for need, t, (a, b) in zip(ctx.needs_input_grad[4:], cond, TABLES):
-            grads.append(dcond[at:at + a * b].view(a, b).to(t.dtype) if need else None)
-            at += a * b
-        return (dlogits, None, None, None, *grads)
+        if torch.is_grad_enabled():   # the gradients' own graph is wanted: they have none, and say so when it is used
+            return once_differentiable(_logp_gradients)(ctx, glp, gent)
+        return _logp_gradients(ctx, glp, gent)
 
 
 def moves_logp(logits, cond, masks, ids, lib_path=None):
@@ -219,9 +234,7 @@ def moves_logp(logits, cond, masks, ids, lib_path=None):
     rows, dev = logits.shape[0], logits.device
     masks = _check_bytes('moves_logp', 'masks', masks, rows, (BYTES,), dev)
     ids = _check_row('moves_logp', 'ids', ids, (rows,), torch.int16, dev)
-    cond = () if cond is None else tuple(cond)
-    if cond and len(cond) != len(TABLES):
-        raise RuntimeError(f'moves_logp: cond must be ten tables, got {len(cond)}')
-    if torch.is_grad_enabled() and (logits.requires_grad or any(t.requires_grad for t in cond)):
+    cond = _check_cond('moves_logp', cond, dev)
+    if torch.is_grad_enabled() and (logits.requires_grad or any([t.requires_grad for t in cond])):
         return _MovesLogp.apply(logits, masks, ids, lib_path, *cond)
-    return _logp_forward(logits, cond or None, masks, ids, lib_path)
+    return _logp_forward(logits, cond, masks, ids, lib_path)

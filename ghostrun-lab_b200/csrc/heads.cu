@@ -24,6 +24,7 @@
 #include <cmath>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 #include "../../include/rlenv_api.h"   // rl_sample, rl_moves_* compiled against their C-ABI declarations
 
 namespace {
@@ -32,7 +33,6 @@ constexpr int kParts = 5, kBytes = 19, kMoves = 324, kTables = 10, kCond = 127;
 constexpr float kScale = 134217728.f;   // 2^27
 constexpr float kUnit = 1.f / kScale;
 constexpr int kThreads = 128;
-constexpr int kRowThreads = 256;
 constexpr int kMaxWidth = 4096;         // 2^12 weights of 2^27 and a u of 2^24 fit 63 bits
 
 thread_local std::string g_heads_error;
@@ -275,185 +275,325 @@ struct RowArgs {
     long long rows;
 };
 
-// A whole number that orders floats as the floats do (-0 as 0; a NaN as -inf); 0 is below all of them.
+// Whole numbers that order values as the values do (-0 as 0, a NaN as -inf), all above 0; 16 bits of them for the 16-bit
+// types, which halves the bisection's steps.
 __device__ __forceinline__ unsigned key_of(float l) {
     if (l != l) l = -INFINITY;
     const unsigned b = __float_as_uint(l + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ unsigned key_of_bits16(unsigned b, unsigned inf) {
+    if ((b & 0x7FFFu) > inf) b = inf | 0x8000u;
+    if (b == 0x8000u) b = 0;
+    return b & 0x8000u ? ~b & 0xFFFFu : b | 0x8000u;
+}
+__device__ __forceinline__ unsigned key_of(__nv_bfloat16 l) { return key_of_bits16(__bfloat16_as_ushort(l), 0x7F80u); }
+__device__ __forceinline__ unsigned key_of(__half l) { return key_of_bits16(__half_as_ushort(l), 0x7C00u); }
+template <class T> __device__ __forceinline__ float value_of(unsigned key);
+template <> __device__ __forceinline__ float value_of<float>(unsigned k) {
+    return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
+template <> __device__ __forceinline__ float value_of<__nv_bfloat16>(unsigned k) {
+    return to_f(__ushort_as_bfloat16(static_cast<unsigned short>(k & 0x8000u ? k & 0x7FFFu : ~k)));
+}
+template <> __device__ __forceinline__ float value_of<__half>(unsigned k) {
+    return to_f(__ushort_as_half(static_cast<unsigned short>(k & 0x8000u ? k & 0x7FFFu : ~k)));
+}
 
-struct BlockSums {
-    unsigned long long part[kRowThreads / 32];
+using u64 = unsigned long long;
+
+// Sums and the like over the TPR threads of a row: one warp's by its reduction instructions, more warps' (one row per
+// block) through shared memory, in two places that take turns, so that one barrier per call is enough.
+template <int TPR>
+struct Team {
+    static constexpr int kWarps = TPR / 32;
+    u64* place;   // [2][kWarps][2]
+    int turn = 0;
+
+    __device__ void exchange(u64& a, u64& b, bool first_is_max) {
+        if constexpr (kWarps > 1) {
+            u64* p = place + turn * kWarps * 2;
+            turn ^= 1;
+            if ((threadIdx.x & 31) == 0) {
+                p[2 * (threadIdx.x >> 5)] = a;
+                p[2 * (threadIdx.x >> 5) + 1] = b;
+            }
+            __syncthreads();
+            a = p[0];
+            b = p[1];
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) {
+                a = first_is_max ? (p[2 * w] > a ? p[2 * w] : a) : a + p[2 * w];
+                b += p[2 * w + 1];
+            }
+        }
+    }
+    // The sums of v and of n.
+    __device__ void sums(unsigned v, unsigned n, u64& total, unsigned& count) {
+        u64 a = static_cast<u64>(__reduce_add_sync(~0u, v & 0xFFFFu)) + (static_cast<u64>(__reduce_add_sync(~0u, v >> 16)) << 16);
+        u64 b = __reduce_add_sync(~0u, n);
+        exchange(a, b, false);
+        total = a;
+        count = static_cast<unsigned>(b);
+    }
+    __device__ u64 sum(unsigned v) {
+        u64 a = static_cast<u64>(__reduce_add_sync(~0u, v & 0xFFFFu)) + (static_cast<u64>(__reduce_add_sync(~0u, v >> 16)) << 16);
+        u64 b = 0;
+        exchange(a, b, false);
+        return a;
+    }
+    // The largest v, and the sum of n.
+    __device__ unsigned largest(unsigned v, unsigned n, unsigned& count) {
+        u64 a = __reduce_max_sync(~0u, v), b = __reduce_add_sync(~0u, n);
+        exchange(a, b, true);
+        count = static_cast<unsigned>(b);
+        return static_cast<unsigned>(a);
+    }
+    // The sum of v over the threads before this one.
+    __device__ u64 before(u64 v) {
+        u64 run = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 up = __shfl_up_sync(~0u, run, o);
+            if ((threadIdx.x & 31) >= o) run += up;
+        }
+        if constexpr (kWarps > 1) {
+            u64* p = place + turn * kWarps * 2;
+            turn ^= 1;
+            if ((threadIdx.x & 31) == 31) p[threadIdx.x >> 5] = run;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w)
+                if (w < static_cast<int>(threadIdx.x >> 5)) run += p[w];
+        }
+        return run - v;
+    }
 };
 
-__device__ __forceinline__ unsigned long long block_sum(unsigned long long v, BlockSums& s) {
+// A row's choices in a thread: four neighbours of each stretch of 4 TPR, so that their order is stretch, thread, place.
+template <int TPR, int EPT>
+struct RowTile {
+    unsigned key[EPT], wgt[EPT];   // 0: not legal, or cut off
+    __device__ static int at(int e) { return (e >> 2) * 4 * TPR + 4 * (static_cast<int>(threadIdx.x) & (TPR - 1)) + (e & 3); }
+};
+
+// Cuts the row to the shortest run of its ranked choices whose amounts (their weights, or 1 each) reach `reach` >= 1, by
+// bisection for the lowest key that stays: what lies above it does not reach. Choices of that key stay by their index.
+// lowest: below all keys of the row; n: how many there are. The row's amounts reach.
+template <bool WEIGHTS, int TPR, int EPT>
+__device__ __forceinline__ void cut_row(RowTile<TPR, EPT>& r, Team<TPR>& team, u64 reach, unsigned top, unsigned lowest, unsigned n) {
+    unsigned lo = lowest, hi = top, n_lo = n, n_hi = 0;   // amounts above lo reach, those above hi do not
+    u64 above = 0;                                        // hi's
+    while (hi - lo > 1 && n_lo - n_hi > 1) {
+        const unsigned mid = lo + (hi - lo) / 2;
+        unsigned v = 0, c = 0;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s.part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    unsigned long long t = 0;
-    for (int w = 0; w < kRowThreads / 32; ++w) t += s.part[w];
-    return t;
+        for (int e = 0; e < EPT; ++e)
+            if (r.key[e] > mid) {
+                if (WEIGHTS) v += r.wgt[e];
+                ++c;
+            }
+        u64 total;
+        if (WEIGHTS) {
+            team.sums(v, c, total, c);
+        } else {
+            total = team.sum(c);
+            c = static_cast<unsigned>(total);
+        }
+        if (total < reach) {
+            hi = mid;
+            n_hi = c;
+            above = total;
+        } else {
+            lo = mid;
+            n_lo = c;
+        }
+    }
+    const unsigned group = n_lo - n_hi;   // all choices in (lo, hi]: one, or several of one key
+    unsigned mine = 0, low = 0, w = 0;
+#pragma unroll
+    for (int e = 0; e < EPT; ++e)
+        if (r.key[e] > lo && r.key[e] <= hi) {
+            low = r.key[e];
+            w = r.wgt[e];
+            ++mine;
+        }
+    unsigned stay = 1;
+    if (group > 1) {
+        unsigned unused;
+        if (WEIGHTS) w = team.largest(w, 0, unused);
+        const u64 left = reach - above, each = WEIGHTS ? w : 1;
+        stay = each == 0 || (left + each - 1) / each >= group ? group : static_cast<unsigned>((left + each - 1) / each);
+    }
+    if (stay < group) {   // the first `stay` of the group by index
+        unsigned past = 0;
+#pragma unroll
+        for (int s = 0; s < EPT / 4; ++s) {
+            unsigned here = 0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) here += r.key[4 * s + q] > lo && r.key[4 * s + q] <= hi;
+            const u64 total = team.sum(here);
+            unsigned rank = past + static_cast<unsigned>(team.before(here));
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (r.key[4 * s + q] > lo && r.key[4 * s + q] <= hi && rank++ >= stay) r.key[4 * s + q] = 0;
+            past += static_cast<unsigned>(total);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < EPT; ++e)
+        if (r.key[e] <= lo) r.key[e] = r.wgt[e] = 0;
 }
 
-__device__ __forceinline__ bool move_legal(const uint8_t* m, int i) {
-    bool ok = m[i % 9] != 0;
-    i /= 9;
-    ok &= m[9 + i % 3] != 0;
-    i /= 3;
-    ok &= m[12 + i % 3] != 0;
-    i /= 3;
-    return ok && m[15 + i % 2] != 0 && m[17 + i / 2] != 0;
-}
-
-// A block per row. The row's keys and weights lie in shared memory; what top-k and top-p keep is a run of the ranked
-// choices, so its lowest key is found by bisection over the key's 32 bits, and the last group of equal keys is cut by index.
-template <class T>
-__global__ void __launch_bounds__(kRowThreads) k_rows_sample(RowArgs a) {
-    extern __shared__ unsigned smem[];
-    __shared__ BlockSums sums;
-    __shared__ unsigned long long scan[kRowThreads];
-    __shared__ int found;
-    unsigned* key = smem;
-    unsigned* wgt = smem + a.width;
-    const int n = a.width, tid = threadIdx.x;
-    const int each = (n + kRowThreads - 1) / kRowThreads;
-    const int lo = min(n, tid * each), hi = min(n, lo + each);   // this thread's stretch in index order
-    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+// A warp, or a block of TPR threads, per row; the row's keys and weights stay in registers. VEC: rows whose four
+// neighbours can be loaded at once.
+template <class T, int TPR, int EPT, bool VEC>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) k_rows_sample(RowArgs a) {
+    constexpr int kTeams = TPR == 32 ? 8 : 1;
+    __shared__ u64 place[4 * Team<TPR>::kWarps];
+    Team<TPR> team;
+    team.place = place;
+    const int n = a.width, lane = threadIdx.x & 31;
+    const bool parts = a.legal && a.legal_width != n;
+    unsigned need[EPT];   // the five mask bytes that a packed move needs, as bits
+    if (parts) {
+#pragma unroll
+        for (int e = 0; e < EPT; ++e) {
+            const int i = RowTile<TPR, EPT>::at(e);
+            need[e] = 1u << i % 9 | 1u << (9 + i / 9 % 3) | 1u << (12 + i / 27 % 3) | 1u << (15 + i / 81 % 2) | 1u << (17 + i / 162 % 2);
+        }
+    }
+    for (long long row = static_cast<long long>(blockIdx.x) * kTeams + (TPR == 32 ? threadIdx.x >> 5 : 0); row < a.rows;
+         row += static_cast<long long>(gridDim.x) * kTeams) {
         const T* logits = static_cast<const T*>(a.logits) + row * a.stride;
         const uint8_t* legal = a.legal ? a.legal + row * a.legal_stride : nullptr;
+        const float u = a.u[row];
         const RowCut q = row_cut(a.cut, row);
-        __syncthreads();   // the previous row's shared memory is free
-        if (tid == 0) found = 0;
-        unsigned top = 0;
-        int any = 0, nan = 0;
-        for (int i = tid; i < n; i += kRowThreads) {
-            const float l = to_f(logits[i]);
-            const bool ok = !legal || (a.legal_width == n ? legal[i] != 0 : move_legal(legal, i));
-            const unsigned k = ok ? key_of(l) : 0u;
-            key[i] = k;
-            top = max(top, k);
-            any |= ok;
-            nan |= ok && l != l;   // chosen as -inf is, and shown in the log-probability
-        }
-        top = __reduce_max_sync(~0u, top);
-        if ((tid & 31) == 0) scan[tid >> 5] = top;
-        any = __syncthreads_or(any);
-        nan = __syncthreads_or(nan);
-        for (int w = 0; w < kRowThreads / 32; ++w) top = max(top, static_cast<unsigned>(scan[w]));
-        const float m = top & 0x80000000u ? __uint_as_float(top & 0x7FFFFFFFu) : __uint_as_float(~top);
-        for (int i = tid; i < n; i += kRowThreads) {
-            float l = to_f(logits[i]);
-            if (l != l) l = -INFINITY;
-            wgt[i] = key[i] ? weight_of(l == m ? 0.f : (l - m) * q.scale) : 0u;
-        }
-        __syncthreads();
-        if (any && q.cut) {
-            if (q.top_k > 0 && q.top_k < n) {
-                // the largest key t with at least k keys >= t, then its group's first by index
-                unsigned t = 0;
-                for (int b = 31; b >= 0; --b) {
-                    const unsigned cand = t | 1u << b;
-                    unsigned long long c = 0;
-                    for (int i = tid; i < n; i += kRowThreads) c += key[i] >= cand;
-                    if (block_sum(c, sums) >= static_cast<unsigned>(q.top_k)) t = cand;
-                }
-                if (t) {
-                    unsigned long long above = 0, mine = 0;
-                    for (int i = lo; i < hi; ++i) {
-                        above += key[i] > t;
-                        mine += key[i] == t;
+        unsigned bits = ~0u;
+        if (parts) bits = __ballot_sync(~0u, lane < kBytes && legal[min(lane, kBytes - 1)] != 0);
+        RowTile<TPR, EPT> r;
+        unsigned top = 0, nans = 0;
+#pragma unroll
+        for (int s = 0; s < EPT / 4; ++s) {
+            const int i = r.at(4 * s);
+            T l[4];
+            uint8_t ok[4];
+            if constexpr (VEC) {
+                if (i < n) {
+                    struct alignas(4 * sizeof(T)) Four { T v[4]; };
+                    const Four f = *reinterpret_cast<const Four*>(logits + i);
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) l[p] = f.v[p];
+                    if (legal && !parts) {
+                        const uchar4 m = *reinterpret_cast<const uchar4*>(legal + i);
+                        ok[0] = m.x;
+                        ok[1] = m.y;
+                        ok[2] = m.z;
+                        ok[3] = m.w;
                     }
-                    above = block_sum(above, sums);
-                    scan[tid] = mine;
-                    __syncthreads();
-                    unsigned long long rank = above;
-                    for (int w = 0; w < tid; ++w) rank += scan[w];
-                    for (int i = lo; i < hi; ++i) {
-                        bool drop = key[i] < t;
-                        if (key[i] == t) drop = rank++ >= static_cast<unsigned>(q.top_k);
-                        if (drop) key[i] = wgt[i] = 0;
-                    }
-                    __syncthreads();
                 }
+            } else {
+#pragma unroll
+                for (int p = 0; p < 4; ++p)
+                    if (i + p < n) {
+                        l[p] = logits[i + p];
+                        if (legal && !parts) ok[p] = legal[i + p];
+                    }
             }
-            unsigned long long s = 0;
-            for (int i = tid; i < n; i += kRowThreads) s += wgt[i];
-            const double reach = static_cast<double>(q.top_p) * static_cast<double>(block_sum(s, sums));
-            // the smallest t for which the weights above t do not reach: what is ranked below the keys >= t goes
-            unsigned t = 0;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                const int e = 4 * s + p;
+                bool in = i + p < n;
+                if (parts) in = in && (bits & need[e]) == need[e];
+                else if (legal) in = in && ok[p] != 0;
+                r.key[e] = in ? key_of(l[p]) : 0u;
+                nans |= in && to_f(l[p]) != to_f(l[p]);
+                top = max(top, r.key[e]);
+            }
+        }
+        top = team.largest(top, nans, nans);
+        if (top == 0) {   // nothing legal
+            if ((threadIdx.x & (TPR - 1)) == 0) {
+                a.choice[row] = 0;
+                a.logp[row] = 0.f;
+            }
+            continue;
+        }
+        const float m = value_of<T>(top);
+        unsigned count = 0, high = 0;   // of the legal choices: how many, and the complement of the lowest key
+#pragma unroll
+        for (int e = 0; e < EPT; ++e) {
+            const float l = value_of<T>(r.key[e]);
+            r.wgt[e] = r.key[e] ? weight_of(l == m ? 0.f : (l - m) * q.scale) : 0u;
+            if (r.key[e]) {
+                ++count;
+                high = max(high, ~r.key[e]);
+            }
+        }
+        if (q.cut) {
+            high = team.largest(high, count, count);
+            if (q.top_k > 0 && static_cast<unsigned>(q.top_k) < count)
+                cut_row<false>(r, team, static_cast<u64>(q.top_k), top, ~high - 1, count);
             if (q.top_p < 1.f) {
-                for (int b = 31; b >= 0; --b) {
-                    const unsigned cand = t | ((1u << b) - 1u);   // the largest value with t's upper bits and this one 0
-                    unsigned long long v = 0;
-                    for (int i = tid; i < n; i += kRowThreads) v += key[i] > cand ? wgt[i] : 0u;
-                    if (!(static_cast<double>(block_sum(v, sums)) < reach)) t |= 1u << b;
+                unsigned w = 0, c = 0;
+                high = 0;
+#pragma unroll
+                for (int e = 0; e < EPT; ++e) {
+                    if (!r.wgt[e]) r.key[e] = 0;   // a choice that weighs nothing adds nothing
+                    w += r.wgt[e];
+                    if (r.key[e]) {
+                        ++c;
+                        high = max(high, ~r.key[e]);
+                    }
                 }
-                if (t > top) t = top;   // p <= 0: the best choice alone
-            }
-            // the lowest key that stays, its group and the weight above it
-            unsigned low = ~0u;
-            for (int i = tid; i < n; i += kRowThreads)
-                if (key[i] && key[i] >= t) low = min(low, key[i]);
-            low = __reduce_min_sync(~0u, low);
-            __syncthreads();
-            if ((tid & 31) == 0) scan[tid >> 5] = low;
-            __syncthreads();
-            for (int w = 0; w < kRowThreads / 32; ++w) low = min(low, static_cast<unsigned>(scan[w]));
-            __syncthreads();
-            unsigned long long above = 0, mine = 0;
-            for (int i = lo; i < hi; ++i) {
-                above += key[i] > low ? wgt[i] : 0u;
-                mine += key[i] == low ? wgt[i] : 0u;
-            }
-            above = block_sum(above, sums);
-            scan[tid] = mine;
-            __syncthreads();
-            unsigned long long run = above;
-            bool first = low == top;   // whether the best choice of all is in this group: the first by index is it
-            for (int w = 0; w < tid; ++w) {
-                run += scan[w];
-                first &= scan[w] == 0;
+                u64 total;
+                team.sums(w, 0, total, count);
+                high = team.largest(high, c, count);
+                const double reach = ceil(static_cast<double>(q.top_p) * static_cast<double>(total));
+                cut_row<true>(r, team, reach < 1.0 ? 1ull : static_cast<u64>(reach), top, ~high - 1, count);
             }
             const double least = static_cast<double>(q.min_p) * static_cast<double>(kScale);
-            for (int i = lo; i < hi; ++i) {
-                bool keep = key[i] >= low;
-                if (key[i] == low) {
-                    if (q.top_p < 1.f) keep = first || static_cast<double>(run) < reach;
-                    first = false;
-                    run += wgt[i];
-                }
-                if (!keep || (key[i] != top && static_cast<double>(wgt[i]) < least)) wgt[i] = 0;
-            }
-            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < EPT; ++e)
+                if (static_cast<double>(r.wgt[e]) < least) r.wgt[e] = 0;
         }
-        unsigned long long mine = 0;
-        for (int i = lo; i < hi; ++i) mine += wgt[i];
-        const unsigned long long total = block_sum(mine, sums);
-        const unsigned long long target = (bits24(a.u[row]) * total) >> 24;
-        scan[tid] = mine;
-        __syncthreads();
-        unsigned long long run = 0;
-        for (int w = 0; w < tid; ++w) run += scan[w];
-        if (run <= target && target < run + mine)
-            for (int i = lo; i < hi; ++i) {
-                run += wgt[i];
-                if (run > target) {
-                    found = i;
-                    break;
+        // the stretch of the row, then the thread, then the place in which the running sum passes the target
+        u64 part[EPT / 4], total = 0;
+#pragma unroll
+        for (int s = 0; s < EPT / 4; ++s) {
+            part[s] = team.sum(r.wgt[4 * s] + r.wgt[4 * s + 1] + r.wgt[4 * s + 2] + r.wgt[4 * s + 3]);
+            total += part[s];
+        }
+        u64 target = (bits24(u) * total) >> 24;
+        int stretch = 0;
+        unsigned w[4] = {r.wgt[0], r.wgt[1], r.wgt[2], r.wgt[3]}, k[4] = {r.key[0], r.key[1], r.key[2], r.key[3]};
+#pragma unroll
+        for (int s = 1; s < EPT / 4; ++s)
+            if (stretch == s - 1 && target >= part[s - 1]) {
+                target -= part[s - 1];
+                stretch = s;
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    w[p] = r.wgt[4 * s + p];
+                    k[p] = r.key[4 * s + p];
                 }
             }
-        __syncthreads();
-        if (tid == 0) {
-            const int c = any ? found : 0;
-            float lp = 0.f;
-            if (any) {
-                const float l = to_f(logits[c]);
-                lp = nan ? NAN : (l == m ? 0.f : (l - m) * q.scale) - logf(static_cast<float>(total) * kUnit);
-            }
-            a.choice[row] = c;
-            a.logp[row] = lp;
+        const u64 own = static_cast<u64>(w[0]) + w[1] + w[2] + w[3], run = team.before(own);
+        if (run <= target && target < run + own) {
+            unsigned left = static_cast<unsigned>(target - run);
+            int c = 0;
+            unsigned key = k[0];
+#pragma unroll
+            for (int p = 0; p < 3; ++p)
+                if (c == p && left >= w[p]) {
+                    left -= w[p];
+                    c = p + 1;
+                    key = k[p + 1];
+                }
+            const float l = value_of<T>(key);
+            const float lp = (l == m ? 0.f : (l - m) * q.scale) - logf(static_cast<float>(total) * kUnit);
+            a.choice[row] = r.at(4 * stretch) + c;
+            a.logp[row] = nans ? NAN : lp;
         }
     }
 }
@@ -669,6 +809,19 @@ bool with_type(int type, F f) {
     return true;
 }
 
+// f of the row's tile (threads per row, choices per thread): the smallest that holds it.
+template <class F>
+void with_row_tile(int width, F f) {
+    using std::integral_constant;
+    if (width <= 128) f(integral_constant<int, 32>{}, integral_constant<int, 4>{});
+    else if (width <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+    else if (width <= 384) f(integral_constant<int, 32>{}, integral_constant<int, 12>{});
+    else if (width <= 512) f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+    else if (width <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
+    else if (width <= 2048) f(integral_constant<int, 128>{}, integral_constant<int, 16>{});
+    else f(integral_constant<int, 256>{}, integral_constant<int, 16>{});
+}
+
 const char* bad_cut(float temperature, const void* temperatures, float top_p, const void* top_ps, float min_p,
                     const void* min_ps) {
     if (!temperatures && !(temperature >= 0.f)) return "temperature must be 0 or more";
@@ -735,10 +888,17 @@ int rl_sample(const void* logits, long long stride, int type, int width, const v
     a.choice = static_cast<long long*>(choice);
     a.logp = static_cast<float*>(logp);
     a.rows = rows;
-    const unsigned grid = blocks_for(rows, 1, 8ll * sm_count());
-    const size_t smem = 2 * sizeof(unsigned) * static_cast<size_t>(width);
+    const size_t e4 = type == 0 ? 16 : 8;   // bytes of four values
+    const bool vec = width % 4 == 0 && stride % 4 == 0 && reinterpret_cast<uintptr_t>(logits) % e4 == 0 &&
+                     (!legal || legal_width != width || (legal_stride % 4 == 0 && reinterpret_cast<uintptr_t>(legal) % 4 == 0));
     with_type(type, [&](auto t) {
-        k_rows_sample<decltype(t)><<<grid, kRowThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
+        using T = decltype(t);
+        with_row_tile(width, [&](auto tpr, auto ept) {
+            const unsigned grid = tpr() == 32 ? blocks_for(rows, 8, 8ll * sm_count()) : blocks_for(rows, 1, 2048ll / tpr() * sm_count());
+            const unsigned block = tpr() == 32 ? 256 : tpr();
+            if (vec) k_rows_sample<T, tpr(), ept(), true><<<grid, block, 0, static_cast<cudaStream_t>(stream)>>>(a);
+            else k_rows_sample<T, tpr(), ept(), false><<<grid, block, 0, static_cast<cudaStream_t>(stream)>>>(a);
+        });
     });
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? 0 : failed(cudaGetErrorString(e));

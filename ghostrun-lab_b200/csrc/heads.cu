@@ -21,6 +21,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <string>
@@ -32,7 +33,8 @@ namespace {
 constexpr int kParts = 5, kBytes = 19, kMoves = 324, kTables = 10, kCond = 127;
 constexpr float kScale = 134217728.f;   // 2^27
 constexpr float kUnit = 1.f / kScale;
-constexpr int kThreads = 128;
+constexpr int kThreads = 128;           // and rows of a block's batch
+constexpr int kDevices = 64;            // whose properties are kept
 constexpr int kMaxWidth = 4096;         // 2^12 weights of 2^27 and a u of 2^24 fit 63 bits
 
 thread_local std::string g_heads_error;
@@ -104,26 +106,58 @@ __device__ __forceinline__ unsigned bits24(float u) {
     return static_cast<unsigned>(min(max(v, 0), 0xFFFFFF));
 }
 
-// All ten tables, in fp32, into shared memory.
+// All ten tables, in fp32, into shared memory: an entry per thread, so that they arrive together.
 __device__ __forceinline__ void load_cond(float* tab, const Cond& c) {
-    if (c.type < 0) return;
+    static_assert(kCond <= kThreads, "an entry per thread");
+    if (c.type < 0 || threadIdx.x >= kCond) return;
+    int t = 0, at = 0;
 #pragma unroll
-    for (int k = 1; k < kParts; ++k)
-#pragma unroll
-        for (int j = 0; j < k; ++j) {
-            const int t = table_of(k, j), n = part_n(j) * part_n(k);
-            for (int i = threadIdx.x; i < n; i += blockDim.x) {
-                const float v = c.type == 0 ? static_cast<const float*>(c.table[t])[i]
-                                : c.type == 1 ? to_f(static_cast<const __nv_bfloat16*>(c.table[t])[i])
-                                              : to_f(static_cast<const __half*>(c.table[t])[i]);
-                tab[table_at(t) + i] = v;
-            }
+    for (int i = 1; i < kTables; ++i)
+        if (static_cast<int>(threadIdx.x) >= table_at(i)) {
+            t = i;
+            at = table_at(i);
         }
+    const int i = static_cast<int>(threadIdx.x) - at;
+    tab[threadIdx.x] = c.type == 0 ? static_cast<const float*>(c.table[t])[i]
+                       : c.type == 1 ? to_f(static_cast<const __nv_bfloat16*>(c.table[t])[i])
+                                     : to_f(static_cast<const __half*>(c.table[t])[i]);
 }
 
-// One choice among the legal ones of N logits; adds its log-probability to lp.
+// ------------------------------------------------------------------ batches of rows in shared memory
+//
+// A block takes kThreads rows at a time, a thread each. A row's 19 logits and 19 mask bytes are no place to start a wide
+// load, but kThreads rows of them are: a block's rows come as one stretch of 16-byte asynchronous copies, one batch ahead.
+// Rows that do not lie end to end from a 16-byte boundary are fetched value by value.
+
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src)
+                 : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
-__device__ __forceinline__ int choose(float (&l)[N], unsigned legal, float u, const RowCut& q, float& lp) {
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Rows [first, first + n) of COLS values each into shared memory, end to end.
+template <int COLS, class T>
+__device__ __forceinline__ void stage(T* dst, const void* base, long long first, int n, long long stride, bool dense) {
+    const T* src = static_cast<const T*>(base) + first * stride;
+    if (dense) {
+        constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+        const int all = n * COLS, whole = all & ~(kPer - 1);
+        for (int i = threadIdx.x * kPer; i < whole; i += kThreads * kPer) copy16(dst + i, src + i);
+        for (int i = whole + threadIdx.x; i < all; i += kThreads) dst[i] = src[i];
+    } else {
+        for (int i = threadIdx.x; i < n * COLS; i += kThreads) {
+            const int row = i / COLS;
+            dst[i] = src[row * stride + (i - row * COLS)];
+        }
+    }
+}
+
+// One choice among the legal ones of N logits; its d is added to d_sum, its total multiplied into totals (d_sum - log totals
+// is the move's log-probability: one logarithm for the five parts).
+template <int N>
+__device__ __forceinline__ int choose(float (&l)[N], unsigned legal, float u, const RowCut& q, float& d_sum, float& totals) {
     if (!legal) return 0;
     float m = -INFINITY;
     bool nan = false;
@@ -158,15 +192,15 @@ __device__ __forceinline__ int choose(float (&l)[N], unsigned legal, float u, co
             if (rank[i] >= top) w[i] = 0;
             total += w[i];
         }
-        const double reach = static_cast<double>(q.top_p) * static_cast<double>(total);
-        const double least = static_cast<double>(q.min_p) * static_cast<double>(kScale);
+        const unsigned reach = static_cast<unsigned>(ceil(static_cast<double>(q.top_p) * static_cast<double>(total)));
+        const unsigned least = static_cast<unsigned>(ceil(static_cast<double>(q.min_p) * static_cast<double>(kScale)));
         unsigned kept = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             unsigned before = 0;
 #pragma unroll
             for (int j = 0; j < N; ++j) before += rank[j] < rank[i] ? w[j] : 0u;
-            const bool keep = rank[i] == 0 || (static_cast<double>(before) < reach && static_cast<double>(w[i]) >= least);
+            const bool keep = rank[i] == 0 || (before < reach && w[i] >= least);
             kept |= static_cast<unsigned>(keep) << i;
         }
 #pragma unroll
@@ -188,7 +222,8 @@ __device__ __forceinline__ int choose(float (&l)[N], unsigned legal, float u, co
         }
         run -= w[i];
     }
-    lp += nan ? NAN : dc - logf(static_cast<float>(total) * kUnit);
+    d_sum += nan ? NAN : dc;
+    totals *= static_cast<float>(total) * kUnit;
     return c;
 }
 
@@ -220,42 +255,69 @@ struct MoveArgs {
     const uint8_t* masks;
     long long mask_stride;
     const float* u;
+    bool dense_logits, dense_masks, dense_u;
     Cut cut;
     int16_t* ids;
     float* logp;
     long long rows;
 };
 
+template <class T>
+struct MoveBatch {
+    T logits[kThreads * kBytes];
+    alignas(16) uint8_t masks[kThreads * kBytes];
+    alignas(16) float u[kThreads * kParts];
+};
+
 template <int K, class T>
-__device__ __forceinline__ void draw_part(const MoveArgs& a, const T* logits, const uint8_t* mask, const float* u,
-                                          const RowCut& q, const float* tab, int* c, float& lp) {
+__device__ __forceinline__ void draw_part(const T* logits, const uint8_t* mask, const float* u, const RowCut& q, const float* tab,
+                                          int* c, float& d_sum, float& totals) {
     float l[part_n(K)];
     part_logits<K>(l, logits, tab, c);
-    c[K] = choose<part_n(K)>(l, part_legal<K>(mask), u[K], q, lp);
+    c[K] = choose<part_n(K)>(l, part_legal<K>(mask), u[K], q, d_sum, totals);
 }
 
 // A thread per row.
 template <class T>
 __global__ void __launch_bounds__(kThreads) k_moves_sample(MoveArgs a) {
+    extern __shared__ __align__(16) unsigned char batches[];
     __shared__ float tab_s[kCond];
+    auto* batch = reinterpret_cast<MoveBatch<T>*>(batches);
+    auto fetch = [&](long long first, MoveBatch<T>& to) {
+        if (first < a.rows) {
+            const int n = static_cast<int>(min(static_cast<long long>(kThreads), a.rows - first));
+            stage<kBytes>(to.logits, a.logits, first, n, a.stride, a.dense_logits);
+            stage<kBytes>(to.masks, a.masks, first, n, a.mask_stride, a.dense_masks);
+            stage<kParts>(to.u, a.u, first, n, kParts, a.dense_u);
+        }
+        copies_commit();
+    };
+    const long long step = static_cast<long long>(gridDim.x) * kThreads;
+    long long first = static_cast<long long>(blockIdx.x) * kThreads;
+    fetch(first, batch[0]);
     load_cond(tab_s, a.cond);
-    __syncthreads();
     const float* tab = a.cond.type < 0 ? nullptr : tab_s;
-    for (long long row = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; row < a.rows;
-         row += static_cast<long long>(gridDim.x) * blockDim.x) {
-        const T* logits = static_cast<const T*>(a.logits) + row * a.stride;
-        const uint8_t* mask = a.masks + row * a.mask_stride;
-        const float* u = a.u + row * kParts;
-        const RowCut q = row_cut(a.cut, row);
-        int c[kParts];
-        float lp = 0.f;
-        draw_part<0>(a, logits, mask, u, q, tab, c, lp);
-        draw_part<1>(a, logits, mask, u, q, tab, c, lp);
-        draw_part<2>(a, logits, mask, u, q, tab, c, lp);
-        draw_part<3>(a, logits, mask, u, q, tab, c, lp);
-        draw_part<4>(a, logits, mask, u, q, tab, c, lp);
-        a.ids[row] = static_cast<int16_t>(c[0] + 9 * c[1] + 27 * c[2] + 81 * c[3] + 162 * c[4]);
-        a.logp[row] = lp;
+    for (int b = 0; first < a.rows; first += step, b ^= 1) {
+        fetch(first + step, batch[b ^ 1]);
+        copies_wait<1>();
+        __syncthreads();
+        const long long row = first + threadIdx.x;
+        if (row < a.rows) {
+            const T* logits = batch[b].logits + threadIdx.x * kBytes;
+            const uint8_t* mask = batch[b].masks + threadIdx.x * kBytes;
+            const float* u = batch[b].u + threadIdx.x * kParts;
+            const RowCut q = row_cut(a.cut, row);
+            int c[kParts];
+            float d_sum = 0.f, totals = 1.f;
+            draw_part<0>(logits, mask, u, q, tab, c, d_sum, totals);
+            draw_part<1>(logits, mask, u, q, tab, c, d_sum, totals);
+            draw_part<2>(logits, mask, u, q, tab, c, d_sum, totals);
+            draw_part<3>(logits, mask, u, q, tab, c, d_sum, totals);
+            draw_part<4>(logits, mask, u, q, tab, c, d_sum, totals);
+            a.ids[row] = static_cast<int16_t>(c[0] + 9 * c[1] + 27 * c[2] + 81 * c[3] + 162 * c[4]);
+            a.logp[row] = d_sum - logf(totals);
+        }
+        __syncthreads();   // the batch may be written again
     }
 }
 
@@ -342,6 +404,11 @@ struct Team {
         exchange(a, b, false);
         return a;
     }
+    __device__ unsigned count(unsigned n) {
+        u64 a = __reduce_add_sync(~0u, n), b = 0;
+        exchange(a, b, false);
+        return static_cast<unsigned>(a);
+    }
     // The largest v, and the sum of n.
     __device__ unsigned largest(unsigned v, unsigned n, unsigned& count) {
         u64 a = __reduce_max_sync(~0u, v), b = __reduce_add_sync(~0u, n);
@@ -379,13 +446,13 @@ struct RowTile {
 
 // Cuts the row to the shortest run of its ranked choices whose amounts (their weights, or 1 each) reach `reach` >= 1, by
 // bisection for the lowest key that stays: what lies above it does not reach. Choices of that key stay by their index.
-// lowest: below all keys of the row; n: how many there are. The row's amounts reach.
+// n: how many choices there are; their amounts reach. guess: where to look first (0: halfway).
 template <bool WEIGHTS, int TPR, int EPT>
-__device__ __forceinline__ void cut_row(RowTile<TPR, EPT>& r, Team<TPR>& team, u64 reach, unsigned top, unsigned lowest, unsigned n) {
-    unsigned lo = lowest, hi = top, n_lo = n, n_hi = 0;   // amounts above lo reach, those above hi do not
-    u64 above = 0;                                        // hi's
+__device__ __forceinline__ void cut_row(RowTile<TPR, EPT>& r, Team<TPR>& team, u64 reach, unsigned top, unsigned guess, unsigned n) {
+    unsigned lo = 0, hi = top, n_lo = n, n_hi = 0;   // amounts above lo reach, those above hi do not
+    u64 above = 0;                                   // hi's
+    unsigned mid = guess > 0 && guess < top ? guess : top / 2;
     while (hi - lo > 1 && n_lo - n_hi > 1) {
-        const unsigned mid = lo + (hi - lo) / 2;
         unsigned v = 0, c = 0;
 #pragma unroll
         for (int e = 0; e < EPT; ++e)
@@ -397,8 +464,8 @@ __device__ __forceinline__ void cut_row(RowTile<TPR, EPT>& r, Team<TPR>& team, u
         if (WEIGHTS) {
             team.sums(v, c, total, c);
         } else {
-            total = team.sum(c);
-            c = static_cast<unsigned>(total);
+            c = team.count(c);
+            total = c;
         }
         if (total < reach) {
             hi = mid;
@@ -408,6 +475,7 @@ __device__ __forceinline__ void cut_row(RowTile<TPR, EPT>& r, Team<TPR>& team, u
             lo = mid;
             n_lo = c;
         }
+        mid = lo + (hi - lo) / 2;
     }
     const unsigned group = n_lo - n_hi;   // all choices in (lo, hi]: one, or several of one key
     unsigned mine = 0, low = 0, w = 0;
@@ -432,12 +500,12 @@ __device__ __forceinline__ void cut_row(RowTile<TPR, EPT>& r, Team<TPR>& team, u
             unsigned here = 0;
 #pragma unroll
             for (int q = 0; q < 4; ++q) here += r.key[4 * s + q] > lo && r.key[4 * s + q] <= hi;
-            const u64 total = team.sum(here);
+            const unsigned total = team.count(here);
             unsigned rank = past + static_cast<unsigned>(team.before(here));
 #pragma unroll
             for (int q = 0; q < 4; ++q)
                 if (r.key[4 * s + q] > lo && r.key[4 * s + q] <= hi && rank++ >= stay) r.key[4 * s + q] = 0;
-            past += static_cast<unsigned>(total);
+            past += total;
         }
     }
 #pragma unroll
@@ -445,22 +513,46 @@ __device__ __forceinline__ void cut_row(RowTile<TPR, EPT>& r, Team<TPR>& team, u
         if (r.key[e] <= lo) r.key[e] = r.wgt[e] = 0;
 }
 
+// Warps per SM that the registers of EPT choices per thread leave room for.
+template <int EPT>
+constexpr int kRowWarps = EPT <= 4 ? 48 : EPT <= 12 ? 32 : 24;
+
+// A key that at least k of the row's choices reach, less one: k / warps of each warp's threads have a choice that reaches the
+// warp's own bound, the lowest of which holds for all. 0 where k is too large for that.
+template <int TPR, int EPT>
+__device__ __forceinline__ unsigned kth_bound(const RowTile<TPR, EPT>& r, Team<TPR>& team, unsigned k) {
+    const unsigned each = (k + Team<TPR>::kWarps - 1) / Team<TPR>::kWarps;
+    if (each > 32) return 0;
+    unsigned best = 0, t = 0;
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) best = max(best, r.key[e]);
+    for (unsigned bit = 1u << (31 - __clz(__reduce_max_sync(~0u, best) | 1u)); bit; bit >>= 1) {
+        const unsigned n = __popc(__ballot_sync(~0u, best >= (t | bit)));
+        if (n >= each) t |= bit;
+        if (n == each) break;
+    }
+    unsigned unused;
+    t = ~team.largest(~t, 0, unused);
+    return t ? t - 1 : 0;
+}
+
 // A warp, or a block of TPR threads, per row; the row's keys and weights stay in registers. VEC: rows whose four
 // neighbours can be loaded at once.
 template <class T, int TPR, int EPT, bool VEC>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) k_rows_sample(RowArgs a) {
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, TPR == 32 ? kRowWarps<EPT> / 8 : kRowWarps<EPT> * 32 / TPR) k_rows_sample(RowArgs a) {
     constexpr int kTeams = TPR == 32 ? 8 : 1;
     __shared__ u64 place[4 * Team<TPR>::kWarps];
     Team<TPR> team;
     team.place = place;
     const int n = a.width, lane = threadIdx.x & 31;
     const bool parts = a.legal && a.legal_width != n;
-    unsigned need[EPT];   // the five mask bytes that a packed move needs, as bits
-    if (parts) {
-#pragma unroll
-        for (int e = 0; e < EPT; ++e) {
-            const int i = RowTile<TPR, EPT>::at(e);
-            need[e] = 1u << i % 9 | 1u << (9 + i / 9 % 3) | 1u << (12 + i / 27 % 3) | 1u << (15 + i / 81 % 2) | 1u << (17 + i / 162 % 2);
+    __shared__ uint4 need_s[TPR == 32 && EPT == 12 ? kMoves / 4 : 1];   // the five mask bytes that a packed move needs, as bits
+    if constexpr (TPR == 32 && EPT == 12) {   // the tile of rows of 324
+        if (parts) {
+            for (int i = threadIdx.x; i < kMoves; i += 256)
+                reinterpret_cast<unsigned*>(need_s)[i] =
+                    1u << i % 9 | 1u << (9 + i / 9 % 3) | 1u << (12 + i / 27 % 3) | 1u << (15 + i / 81 % 2) | 1u << (17 + i / 162);
+            __syncthreads();
         }
     }
     for (long long row = static_cast<long long>(blockIdx.x) * kTeams + (TPR == 32 ? threadIdx.x >> 5 : 0); row < a.rows;
@@ -500,12 +592,21 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) k_rows_sample(RowArgs a
                         if (legal && !parts) ok[p] = legal[i + p];
                     }
             }
+            unsigned need[4] = {0, 0, 0, 0};
+            if constexpr (TPR == 32 && EPT == 12) {
+                if (parts && i < n) {
+                    const uint4 v = need_s[i >> 2];
+                    need[0] = v.x;
+                    need[1] = v.y;
+                    need[2] = v.z;
+                    need[3] = v.w;
+                }
+            }
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
                 const int e = 4 * s + p;
-                bool in = i + p < n;
-                if (parts) in = in && (bits & need[e]) == need[e];
-                else if (legal) in = in && ok[p] != 0;
+                bool in = i + p < n && (bits & need[p]) == need[p];
+                if (legal && !parts) in = in && ok[p] != 0;
                 r.key[e] = in ? key_of(l[p]) : 0u;
                 nans |= in && to_f(l[p]) != to_f(l[p]);
                 top = max(top, r.key[e]);
@@ -520,42 +621,43 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) k_rows_sample(RowArgs a
             continue;
         }
         const float m = value_of<T>(top);
-        unsigned count = 0, high = 0;   // of the legal choices: how many, and the complement of the lowest key
+        unsigned mine = 0;   // legal choices
 #pragma unroll
         for (int e = 0; e < EPT; ++e) {
             const float l = value_of<T>(r.key[e]);
             r.wgt[e] = r.key[e] ? weight_of(l == m ? 0.f : (l - m) * q.scale) : 0u;
-            if (r.key[e]) {
-                ++count;
-                high = max(high, ~r.key[e]);
-            }
+            mine += r.key[e] != 0;
         }
-        if (q.cut) {
-            high = team.largest(high, count, count);
-            if (q.top_k > 0 && static_cast<unsigned>(q.top_k) < count)
-                cut_row<false>(r, team, static_cast<u64>(q.top_k), top, ~high - 1, count);
-            if (q.top_p < 1.f) {
-                unsigned w = 0, c = 0;
-                high = 0;
+        if (q.top_k > 0) {
+            const unsigned k = static_cast<unsigned>(q.top_k), count = team.count(mine);
+            if (k < count) cut_row<false>(r, team, k, top, kth_bound(r, team, k), count);
+        }
+        if (q.top_p < 1.f) {
+            unsigned w = 0, count = 0;
 #pragma unroll
-                for (int e = 0; e < EPT; ++e) {
-                    if (!r.wgt[e]) r.key[e] = 0;   // a choice that weighs nothing adds nothing
-                    w += r.wgt[e];
-                    if (r.key[e]) {
-                        ++c;
-                        high = max(high, ~r.key[e]);
-                    }
-                }
-                u64 total;
-                team.sums(w, 0, total, count);
-                high = team.largest(high, c, count);
-                const double reach = ceil(static_cast<double>(q.top_p) * static_cast<double>(total));
-                cut_row<true>(r, team, reach < 1.0 ? 1ull : static_cast<u64>(reach), top, ~high - 1, count);
+            for (int e = 0; e < EPT; ++e) {
+                if (!r.wgt[e]) r.key[e] = 0;   // a choice that weighs nothing adds nothing
+                w += r.wgt[e];
+                count += r.key[e] != 0;
             }
-            const double least = static_cast<double>(q.min_p) * static_cast<double>(kScale);
+            u64 total;
+            team.sums(w, count, total, count);
+            const double p = ceil(static_cast<double>(q.top_p) * static_cast<double>(total));
+            const u64 reach = p < 1.0 ? 1ull : static_cast<u64>(p);
+            // choices that could all go together are below the lowest key that stays: look at the best of them first
+            const float least = static_cast<float>(total - reach) / static_cast<float>(count);
+            unsigned guess = 0, unused;
 #pragma unroll
             for (int e = 0; e < EPT; ++e)
-                if (static_cast<double>(r.wgt[e]) < least) r.wgt[e] = 0;
+                if (static_cast<float>(r.wgt[e]) <= least) guess = max(guess, r.key[e]);
+            guess = team.largest(guess, 0, unused);
+            cut_row<true>(r, team, reach, top, guess, count);
+        }
+        if (q.min_p > 0.f) {
+            const unsigned least = static_cast<unsigned>(ceil(static_cast<double>(q.min_p) * static_cast<double>(kScale)));
+#pragma unroll
+            for (int e = 0; e < EPT; ++e)
+                if (r.wgt[e] < least) r.wgt[e] = 0;
         }
         // the stretch of the row, then the thread, then the place in which the running sum passes the target
         u64 part[EPT / 4], total = 0;
@@ -606,6 +708,7 @@ struct LogpArgs {
     Cond cond;
     const uint8_t* masks;
     long long mask_stride;
+    bool dense_logits, dense_masks, dense_out;
     const int16_t* ids;
     float *logp, *entropy;               // forward
     const float *glp, *gent;             // backward: incoming gradients, either may be null
@@ -615,10 +718,27 @@ struct LogpArgs {
     long long rows;
 };
 
-// A part's softmax over its legal choices: weights exp(l - m), their sum, l - m.
+template <class T>
+struct LogpBatch {
+    T logits[kThreads * kBytes];
+    alignas(16) uint8_t masks[kThreads * kBytes];
+};
+
+template <class T>
+__device__ __forceinline__ void fetch_batch(const LogpArgs& a, long long first, LogpBatch<T>& to) {
+    if (first < a.rows) {
+        const int n = static_cast<int>(min(static_cast<long long>(kThreads), a.rows - first));
+        stage<kBytes>(to.logits, a.logits, first, n, a.stride, a.dense_logits);
+        stage<kBytes>(to.masks, a.masks, first, n, a.mask_stride, a.dense_masks);
+    }
+    copies_commit();
+}
+
+// A part's softmax over its legal choices: l - m, exp(l - m), their sum, and sum w (l - m) / S: log p = d - log S and the
+// entropy is log S - mean_d, so log p + H = d - mean_d needs no logarithm.
 template <int N>
 struct Soft {
-    float d[N], w[N], sum, log_sum;
+    float d[N], w[N], sum, inv, mean_d;
     unsigned legal;
 };
 
@@ -633,27 +753,22 @@ __device__ __forceinline__ void soft_part(Soft<part_n(K)>& s, const T* logits, c
     for (int i = 0; i < N; ++i)
         if (s.legal >> i & 1) m = fmaxf(m, s.d[i]);
     s.sum = 0.f;
+    float t = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         s.d[i] = s.d[i] == m ? 0.f : s.d[i] - m;
         s.w[i] = s.legal >> i & 1 ? expf(s.d[i]) : 0.f;
         s.sum += s.w[i];
-    }
-    s.log_sum = logf(s.sum);
-}
-
-template <int N>
-__device__ __forceinline__ float entropy_of(const Soft<N>& s) {
-    float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
         if (s.w[i] != 0.f) t = fmaf(s.w[i], s.d[i], t);
-    return s.log_sum - __fdiv_rn(t, s.sum);
+    }
+    s.inv = __frcp_rn(s.sum);
+    s.mean_d = t * s.inv;
 }
 
+// Adds the choice's d, and mean_d, and multiplies the sum in: one logarithm for the five parts.
 template <int K, class T>
-__device__ __forceinline__ void logp_part(const T* logits, const uint8_t* mask, const float* tab, const int* c, float& lp,
-                                          float& ent) {
+__device__ __forceinline__ void logp_part(const T* logits, const uint8_t* mask, const float* tab, const int* c, float& d_sum,
+                                          float& mean_sum, float& sums) {
     constexpr int N = part_n(K);
     Soft<N> s;
     soft_part<K>(s, logits, mask, tab, c);
@@ -662,100 +777,146 @@ __device__ __forceinline__ void logp_part(const T* logits, const uint8_t* mask, 
 #pragma unroll
     for (int i = 0; i < N; ++i)
         if (i == c[K] && (s.legal >> i & 1)) dc = s.d[i];
-    lp += dc - s.log_sum;
-    ent += entropy_of<N>(s);
+    d_sum += dc;
+    mean_sum += s.mean_d;
+    sums *= s.sum;
 }
 
 __device__ __forceinline__ bool parts_of(int id, int* c) {
+    const bool known = id >= 0 && id < kMoves;
+    if (!known) id = 0;
     c[0] = id % 9;
     c[1] = id / 9 % 3;
     c[2] = id / 27 % 3;
     c[3] = id / 81 % 2;
     c[4] = id / 162;
-    return id >= 0 && id < kMoves;
+    return known;
 }
 
 template <class T>
 __global__ void __launch_bounds__(kThreads) k_moves_logp(LogpArgs a) {
+    extern __shared__ __align__(16) unsigned char batches[];
     __shared__ float tab_s[kCond];
+    auto* batch = reinterpret_cast<LogpBatch<T>*>(batches);
+    const long long step = static_cast<long long>(gridDim.x) * kThreads;
+    long long first = static_cast<long long>(blockIdx.x) * kThreads;
+    fetch_batch(a, first, batch[0]);
     load_cond(tab_s, a.cond);
-    __syncthreads();
     const float* tab = a.cond.type < 0 ? nullptr : tab_s;
-    for (long long row = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; row < a.rows;
-         row += static_cast<long long>(gridDim.x) * blockDim.x) {
-        int c[kParts];
-        float lp = 0.f, ent = 0.f;
-        if (parts_of(a.ids[row], c)) {
-            const T* logits = static_cast<const T*>(a.logits) + row * a.stride;
-            const uint8_t* mask = a.masks + row * a.mask_stride;
-            logp_part<0>(logits, mask, tab, c, lp, ent);
-            logp_part<1>(logits, mask, tab, c, lp, ent);
-            logp_part<2>(logits, mask, tab, c, lp, ent);
-            logp_part<3>(logits, mask, tab, c, lp, ent);
-            logp_part<4>(logits, mask, tab, c, lp, ent);
-        } else {
-            lp = ent = NAN;   // no move has this id
+    for (int b = 0; first < a.rows; first += step, b ^= 1) {
+        fetch_batch(a, first + step, batch[b ^ 1]);
+        const long long row = first + threadIdx.x;
+        const int id = row < a.rows ? a.ids[row] : 0;
+        copies_wait<1>();
+        __syncthreads();
+        if (row < a.rows) {
+            int c[kParts];
+            const bool known = parts_of(id, c);   // else no move has this id
+            const T* logits = batch[b].logits + threadIdx.x * kBytes;
+            const uint8_t* mask = batch[b].masks + threadIdx.x * kBytes;
+            float d_sum = 0.f, mean_sum = 0.f, sums = 1.f;
+            logp_part<0>(logits, mask, tab, c, d_sum, mean_sum, sums);
+            logp_part<1>(logits, mask, tab, c, d_sum, mean_sum, sums);
+            logp_part<2>(logits, mask, tab, c, d_sum, mean_sum, sums);
+            logp_part<3>(logits, mask, tab, c, d_sum, mean_sum, sums);
+            logp_part<4>(logits, mask, tab, c, d_sum, mean_sum, sums);
+            const float log_sums = logf(sums);
+            a.logp[row] = known ? d_sum - log_sums : NAN;
+            a.entropy[row] = known ? log_sums - mean_sum : NAN;
         }
-        a.logp[row] = lp;
-        a.entropy[row] = ent;
+        __syncthreads();   // the batch may be written again
     }
 }
 
-// acc: this thread's own column of the block's table sums, kThreads apart.
+// dl = ga 1[i = c] - p (ga + gb (d - mean_d)), in the logits' place; acc: this thread's own column of the block's table
+// sums, kThreads apart (no two of the additions of a part go to one place, so they are read and written together).
 template <int K, class T>
-__device__ __forceinline__ void grad_part(const T* logits, const uint8_t* mask, const float* tab, const int* c, float ga,
-                                          float gb, T* dl, float* acc) {
+__device__ __forceinline__ void grad_part(T* logits, const uint8_t* mask, const float* tab, const int* c, float ga, float gb,
+                                          float* acc) {
     constexpr int N = part_n(K);
     Soft<N> s;
     soft_part<K>(s, logits, mask, tab, c);
-    const float h = s.legal ? entropy_of<N>(s) : 0.f;
+    float g[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        float g = 0.f;
-        if (s.legal >> i & 1) {
-            const float p = __fdiv_rn(s.w[i], s.sum);
-            g = ga * ((i == c[K] ? 1.f : 0.f) - p);
-            if (p != 0.f) g -= gb * p * (s.d[i] - s.log_sum + h);
-        }
-        if (dl) dl[part_at(K) + i] = from_f<T>(g);
+        const float p = s.w[i] * s.inv;
+        g[i] = i == c[K] ? ga : 0.f;
+        if (p != 0.f) g[i] = fmaf(-p, fmaf(gb, s.d[i] - s.mean_d, ga), g[i]);
+        if (!(s.legal >> i & 1)) g[i] = 0.f;
+    }
+    if constexpr (K > 0) {
         if (acc) {
+            float sum[K * N];
 #pragma unroll
-            for (int j = 0; j < K; ++j) acc[(table_at(table_of(K, j)) + c[j] * N + i) * kThreads] += g;
+            for (int j = 0; j < K; ++j)
+#pragma unroll
+                for (int i = 0; i < N; ++i) sum[j * N + i] = acc[(table_at(table_of(K, j)) + c[j] * N + i) * kThreads] + g[i];
+#pragma unroll
+            for (int j = 0; j < K; ++j)
+#pragma unroll
+                for (int i = 0; i < N; ++i) acc[(table_at(table_of(K, j)) + c[j] * N + i) * kThreads] = sum[j * N + i];
         }
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i) logits[part_at(K) + i] = from_f<T>(g[i]);
 }
 
 // A thread per row; every thread sums the tables' gradient in a column of its own of shared memory, so that no two add
 // to one place and the order of the additions is the launch's alone.
 template <class T>
 __global__ void __launch_bounds__(kThreads) k_moves_grad(LogpArgs a) {
-    extern __shared__ float acc_s[];
+    extern __shared__ __align__(16) unsigned char batches[];   // two batches, then [127][kThreads] sums
     __shared__ float tab_s[kCond];
+    auto* batch = reinterpret_cast<LogpBatch<T>*>(batches);
+    float* acc_s = reinterpret_cast<float*>(batches + 2 * sizeof(LogpBatch<T>));
+    const long long step = static_cast<long long>(gridDim.x) * kThreads;
+    long long first = static_cast<long long>(blockIdx.x) * kThreads;
+    fetch_batch(a, first, batch[0]);
     load_cond(tab_s, a.cond);
     float* acc = a.part ? acc_s + threadIdx.x : nullptr;
     if (acc)
         for (int e = 0; e < kCond; ++e) acc[e * kThreads] = 0.f;
-    __syncthreads();
     const float* tab = a.cond.type < 0 ? nullptr : tab_s;
-    for (long long row = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; row < a.rows;
-         row += static_cast<long long>(gridDim.x) * blockDim.x) {
-        int c[kParts];
-        T* dl = a.dlogits ? static_cast<T*>(a.dlogits) + row * kBytes : nullptr;
-        if (parts_of(a.ids[row], c)) {
-            const T* logits = static_cast<const T*>(a.logits) + row * a.stride;
-            const uint8_t* mask = a.masks + row * a.mask_stride;
-            const float ga = a.glp ? a.glp[row * a.glp_stride] : 0.f, gb = a.gent ? a.gent[row * a.gent_stride] : 0.f;
-            grad_part<0>(logits, mask, tab, c, ga, gb, dl, acc);
-            grad_part<1>(logits, mask, tab, c, ga, gb, dl, acc);
-            grad_part<2>(logits, mask, tab, c, ga, gb, dl, acc);
-            grad_part<3>(logits, mask, tab, c, ga, gb, dl, acc);
-            grad_part<4>(logits, mask, tab, c, ga, gb, dl, acc);
-        } else if (dl) {
-            for (int i = 0; i < kBytes; ++i) dl[i] = from_f<T>(0.f);
+    for (int b = 0; first < a.rows; first += step, b ^= 1) {
+        fetch_batch(a, first + step, batch[b ^ 1]);
+        const long long row = first + threadIdx.x;
+        int id = 0;
+        float ga = 0.f, gb = 0.f;
+        if (row < a.rows) {
+            id = a.ids[row];
+            if (a.glp) ga = a.glp[row * a.glp_stride];
+            if (a.gent) gb = a.gent[row * a.gent_stride];
         }
+        copies_wait<1>();
+        __syncthreads();
+        T* logits = batch[b].logits;
+        if (row < a.rows) {
+            int c[kParts];
+            T* l = logits + threadIdx.x * kBytes;
+            if (parts_of(id, c)) {
+                const uint8_t* mask = batch[b].masks + threadIdx.x * kBytes;
+                grad_part<0>(l, mask, tab, c, ga, gb, acc);
+                grad_part<1>(l, mask, tab, c, ga, gb, acc);
+                grad_part<2>(l, mask, tab, c, ga, gb, acc);
+                grad_part<3>(l, mask, tab, c, ga, gb, acc);
+                grad_part<4>(l, mask, tab, c, ga, gb, acc);
+            } else {
+                for (int i = 0; i < kBytes; ++i) l[i] = from_f<T>(0.f);
+            }
+        }
+        __syncthreads();
+        if (a.dlogits) {
+            const int n = static_cast<int>(min(static_cast<long long>(kThreads), a.rows - first)) * kBytes;
+            T* out = static_cast<T*>(a.dlogits) + first * kBytes;
+            constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+            const int whole = a.dense_out ? n & ~(kPer - 1) : 0;
+            for (int i = threadIdx.x * kPer; i < whole; i += kThreads * kPer)
+                *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<const uint4*>(logits + i);
+            for (int i = whole + threadIdx.x; i < n; i += kThreads) out[i] = logits[i];
+        }
+        __syncthreads();   // the batch may be written again
     }
     if (!a.part) return;
-    __syncthreads();
     if (threadIdx.x < kCond) {
         float t = 0.f;
         for (int j = 0; j < kThreads; ++j) t += acc_s[threadIdx.x * kThreads + (j + threadIdx.x) % kThreads];
@@ -772,14 +933,43 @@ __global__ void __launch_bounds__(32) k_moves_grad_sum(const float* part, int bl
     if (threadIdx.x == 0) dcond[blockIdx.x] = t;
 }
 
-constexpr size_t kGradSmem = static_cast<size_t>(kCond) * kThreads * sizeof(float);
+constexpr int kGradBlocks = 2;   // per SM: each has 65 KB of table sums
+constexpr size_t kGradSums = static_cast<size_t>(kCond) * kThreads * sizeof(float);
 
+int current_device() {
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess ? dev : -1;
+}
+
+// The current device's SM count, asked once per device.
 int sm_count() {
-    int dev = 0, sms = 148;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    static std::atomic<int> known[kDevices];
+    const int dev = current_device();
+    const bool kept = dev >= 0 && dev < kDevices;
+    int sms = kept ? known[dev].load(std::memory_order_relaxed) : 0;
+    if (sms > 0) return sms;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1) return 148;
+    if (kept) known[dev].store(sms, std::memory_order_relaxed);
     return sms;
 }
+
+// Launches a kernel that may need more shared memory than the 48 KB it has unasked (asked for once per device).
+template <auto KERNEL, class A>
+cudaError_t launch(unsigned grid, size_t smem, cudaStream_t stream, const A& a) {
+    static std::atomic<bool> asked[kDevices];
+    if (smem > 48 * 1024) {
+        const int dev = current_device();
+        if (dev < 0 || dev >= kDevices || !asked[dev].load(std::memory_order_acquire)) {
+            const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+            if (e != cudaSuccess) return e;
+            if (dev >= 0 && dev < kDevices) asked[dev].store(true, std::memory_order_release);
+        }
+    }
+    KERNEL<<<grid, kThreads, smem, stream>>>(a);
+    return cudaSuccess;
+}
+
+bool dense(const void* p, bool end_to_end) { return end_to_end && reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 unsigned blocks_for(long long rows, long long per_block, long long most) {
     const long long n = (rows + per_block - 1) / per_block;
@@ -857,8 +1047,14 @@ int rl_moves_sample(const void* logits, long long stride, int type, const void* 
     a.ids = static_cast<int16_t*>(ids);
     a.logp = static_cast<float*>(logp);
     a.rows = rows;
-    const unsigned grid = blocks_for(rows, kThreads, 16ll * sm_count());
-    with_type(type, [&](auto t) { k_moves_sample<decltype(t)><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(a); });
+    a.dense_logits = dense(logits, stride == kBytes);
+    a.dense_masks = dense(masks, mask_stride == kBytes);
+    a.dense_u = dense(u, true);
+    const unsigned grid = blocks_for(rows, kThreads, 6ll * sm_count());
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        k_moves_sample<T><<<grid, kThreads, 2 * sizeof(MoveBatch<T>), static_cast<cudaStream_t>(stream)>>>(a);
+    });
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? 0 : failed(cudaGetErrorString(e));
 }
@@ -894,7 +1090,8 @@ int rl_sample(const void* logits, long long stride, int type, int width, const v
     with_type(type, [&](auto t) {
         using T = decltype(t);
         with_row_tile(width, [&](auto tpr, auto ept) {
-            const unsigned grid = tpr() == 32 ? blocks_for(rows, 8, 8ll * sm_count()) : blocks_for(rows, 1, 2048ll / tpr() * sm_count());
+            const unsigned grid = tpr() == 32 ? blocks_for(rows, 8, kRowWarps<ept()> / 8ll * sm_count())
+                                              : blocks_for(rows, 1, kRowWarps<ept()> * 32ll / tpr() * sm_count());
             const unsigned block = tpr() == 32 ? 256 : tpr();
             if (vec) k_rows_sample<T, tpr(), ept(), true><<<grid, block, 0, static_cast<cudaStream_t>(stream)>>>(a);
             else k_rows_sample<T, tpr(), ept(), false><<<grid, block, 0, static_cast<cudaStream_t>(stream)>>>(a);
@@ -921,13 +1118,18 @@ int rl_moves_logp(const void* logits, long long stride, int type, const void* co
     a.logp = static_cast<float*>(logp);
     a.entropy = static_cast<float*>(entropy);
     a.rows = rows;
-    const unsigned grid = blocks_for(rows, kThreads, 16ll * sm_count());
-    with_type(type, [&](auto t) { k_moves_logp<decltype(t)><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(a); });
+    a.dense_logits = dense(logits, stride == kBytes);
+    a.dense_masks = dense(masks, mask_stride == kBytes);
+    const unsigned grid = blocks_for(rows, kThreads, 8ll * sm_count());
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        k_moves_logp<T><<<grid, kThreads, 2 * sizeof(LogpBatch<T>), static_cast<cudaStream_t>(stream)>>>(a);
+    });
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? 0 : failed(cudaGetErrorString(e));
 }
 
-size_t rl_moves_logp_bwd_work_bytes(void) { return static_cast<size_t>(3) * sm_count() * kCond * sizeof(float); }
+size_t rl_moves_logp_bwd_work_bytes(void) { return static_cast<size_t>(kGradBlocks) * sm_count() * kCond * sizeof(float); }
 
 int rl_moves_logp_bwd(const void* glp, long long glp_stride, const void* gent, long long gent_stride, const void* logits,
                       long long stride, int type, const void* const* cond, int cond_type, const void* masks,
@@ -953,14 +1155,15 @@ int rl_moves_logp_bwd(const void* glp, long long glp_stride, const void* gent, l
     a.dlogits = dlogits;
     a.part = dcond ? static_cast<float*>(work) : nullptr;
     a.rows = rows;
-    const unsigned grid = blocks_for(rows, kThreads, 3ll * sm_count());
-    const size_t smem = dcond ? kGradSmem : 0;
+    a.dense_logits = dense(logits, stride == kBytes);
+    a.dense_masks = dense(masks, mask_stride == kBytes);
+    a.dense_out = dense(dlogits, true);
+    const unsigned grid = blocks_for(rows, kThreads, static_cast<long long>(kGradBlocks) * sm_count());
     auto s = static_cast<cudaStream_t>(stream);
     cudaError_t e = cudaSuccess;
     with_type(type, [&](auto t) {
-        auto k = k_moves_grad<decltype(t)>;
-        e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kGradSmem));
-        if (e == cudaSuccess) k<<<grid, kThreads, smem, s>>>(a);
+        using T = decltype(t);
+        e = launch<k_moves_grad<T>>(grid, 2 * sizeof(LogpBatch<T>) + (dcond ? kGradSums : 0), s, a);
     });
     if (e == cudaSuccess) e = cudaGetLastError();
     if (e == cudaSuccess && dcond) {

@@ -90,7 +90,7 @@ __device__ __forceinline__ RowCut row_cut(const Cut& c, long long row) {
     r.min_p = r.min_p > 0.f ? fminf(r.min_p, 1.f) : 0.f;
     if (r.top_k < 0) r.top_k = 0;
     r.scale = __fdiv_rn(1.f, t);
-    if (!(t > 0.f)) {   // 0 (or nothing a temperature can be): the best choice alone
+    if (!(t > 0.f) || r.scale == INFINITY) {   // 0 (or nothing a temperature can be): the best choice alone
         r.top_k = 1;
         r.scale = 1.f;
     }
@@ -98,8 +98,15 @@ __device__ __forceinline__ RowCut row_cut(const Cut& c, long long row) {
     return r;
 }
 
-// W of a scaled logit d <= 0 (a NaN, -inf at an infinite temperature, weighs nothing).
-__device__ __forceinline__ unsigned weight_of(float d) { return d <= 0.f ? __float2uint_rn(expf(d) * kScale) : 0u; }
+// W of a scaled logit d <= 0 (-inf, and the NaN of -inf at an infinite temperature, weigh nothing).
+__device__ __forceinline__ unsigned weight_of(float d) { return __float2uint_rn(expf(d) * kScale); }
+
+// The larger of two; a NaN if either is one.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 
 __device__ __forceinline__ unsigned bits24(float u) {
     const int v = static_cast<int>(u * 16777216.f);   // a NaN is 0
@@ -154,27 +161,49 @@ __device__ __forceinline__ void stage(T* dst, const void* base, long long first,
     }
 }
 
-// One choice among the legal ones of N logits; its d is added to d_sum, its total multiplied into totals (d_sum - log totals
-// is the move's log-probability: one logarithm for the five parts).
+// Logits of a part whose largest legal one is not finite, brought to the case where it is: what equals it (or, for -inf, what
+// is legal at all) becomes 0, the rest -inf. A NaN is taken as -inf. False where nothing is legal.
 template <int N>
-__device__ __forceinline__ int choose(float (&l)[N], unsigned legal, float u, const RowCut& q, float& d_sum, float& totals) {
-    if (!legal) return 0;
-    float m = -INFINITY;
-    bool nan = false;
-#pragma unroll
+__device__ __noinline__ bool settle(float* l, const uint8_t* mask, float& m) {
+    m = -INFINITY;
+    bool any = false;
     for (int i = 0; i < N; ++i) {
-        if (l[i] != l[i]) {   // a NaN is chosen as -inf is, and shows in the log-probability
-            nan |= legal >> i & 1;
-            l[i] = -INFINITY;
-        }
-        if (legal >> i & 1) m = fmaxf(m, l[i]);
+        m = fmaxf(m, l[i]);
+        any |= mask[i] != 0;
+    }
+    if (fabsf(m) < INFINITY) {   // there was a NaN
+        for (int i = 0; i < N; ++i)
+            if (l[i] != l[i]) l[i] = -INFINITY;
+        return any;
+    }
+    for (int i = 0; i < N; ++i) l[i] = mask[i] != 0 && (m < 0.f ? !(l[i] > m) : l[i] == m) ? 0.f : -INFINITY;
+    m = 0.f;
+    return any;
+}
+
+// One choice of N logits (-inf: not legal); its d is added to d_sum, its total multiplied into totals (d_sum - log totals is
+// the move's log-probability: one logarithm for the five parts).
+template <int N>
+__device__ __forceinline__ int choose(float (&l)[N], const uint8_t* mask, float u, const RowCut& q, float& d_sum, float& totals) {
+    float m = l[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = max_nan(m, l[i]);
+    bool nan = false;
+    if (!(fabsf(m) < INFINITY)) {
+        nan = m != m;
+        float v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = l[i];
+        if (!settle<N>(v, mask, m)) return 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) l[i] = v[i];
     }
     float d[N];
     unsigned w[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        d[i] = l[i] == m ? 0.f : (l[i] - m) * q.scale;
-        w[i] = legal >> i & 1 ? weight_of(d[i]) : 0u;
+        d[i] = (l[i] - m) * q.scale;
+        w[i] = weight_of(d[i]);
     }
     if (q.cut) {
         int rank[N];
@@ -183,7 +212,7 @@ __device__ __forceinline__ int choose(float (&l)[N], unsigned legal, float u, co
             rank[i] = 0;
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                rank[i] += j != i && (legal >> j & 1) && (l[j] > l[i] || (j < i && !(l[i] > l[j])));
+                if (j != i) rank[i] += j < i ? l[j] >= l[i] : l[j] > l[i];
         }
         const int top = q.top_k > 0 ? q.top_k : N;
         unsigned total = 0;
@@ -227,9 +256,10 @@ __device__ __forceinline__ int choose(float (&l)[N], unsigned legal, float u, co
     return c;
 }
 
-// Part K's logits of a row whose earlier choices are c[0..K).
+// Part K's logits of a row whose earlier choices are c[0..K); -inf where the mask says so.
 template <int K, class T>
-__device__ __forceinline__ void part_logits(float (&l)[part_n(K)], const T* logits, const float* tab, const int* c) {
+__device__ __forceinline__ void part_logits(float (&l)[part_n(K)], const T* logits, const uint8_t* mask, const float* tab,
+                                            const int* c) {
 #pragma unroll
     for (int i = 0; i < part_n(K); ++i) l[i] = to_f(logits[part_at(K) + i]);
     if (tab) {
@@ -238,14 +268,8 @@ __device__ __forceinline__ void part_logits(float (&l)[part_n(K)], const T* logi
 #pragma unroll
             for (int i = 0; i < part_n(K); ++i) l[i] += tab[table_at(table_of(K, j)) + c[j] * part_n(K) + i];
     }
-}
-
-template <int K>
-__device__ __forceinline__ unsigned part_legal(const uint8_t* mask) {
-    unsigned m = 0;
 #pragma unroll
-    for (int i = 0; i < part_n(K); ++i) m |= static_cast<unsigned>(mask[part_at(K) + i] != 0) << i;
-    return m;
+    for (int i = 0; i < part_n(K); ++i) l[i] = mask[part_at(K) + i] != 0 ? l[i] : -INFINITY;
 }
 
 struct MoveArgs {
@@ -273,8 +297,8 @@ template <int K, class T>
 __device__ __forceinline__ void draw_part(const T* logits, const uint8_t* mask, const float* u, const RowCut& q, const float* tab,
                                           int* c, float& d_sum, float& totals) {
     float l[part_n(K)];
-    part_logits<K>(l, logits, tab, c);
-    c[K] = choose<part_n(K)>(l, part_legal<K>(mask), u[K], q, d_sum, totals);
+    part_logits<K>(l, logits, mask, tab, c);
+    c[K] = choose<part_n(K)>(l, mask + part_at(K), u[K], q, d_sum, totals);
 }
 
 // A thread per row.
@@ -337,20 +361,18 @@ struct RowArgs {
     long long rows;
 };
 
-// Whole numbers that order values as the values do (-0 as 0, a NaN as -inf), all above 0; 16 bits of them for the 16-bit
-// types, which halves the bisection's steps.
-__device__ __forceinline__ unsigned key_of(float l) {
-    if (l != l) l = -INFINITY;
-    const unsigned b = __float_as_uint(l + 0.f);
+// Whole numbers that order the values of a type as the values do, 16 bits of them for the 16-bit types (which halves the
+// bisection's steps), and back. No NaN comes here; -0 and 0 differ, which the bisection's comparisons, of values, do not see.
+__device__ __forceinline__ unsigned order16(unsigned b) { return b & 0x8000u ? ~b & 0xFFFFu : b | 0x8000u; }
+template <class T> __device__ __forceinline__ unsigned key_of(float l);
+template <> __device__ __forceinline__ unsigned key_of<float>(float l) {
+    const unsigned b = __float_as_uint(l);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ unsigned key_of_bits16(unsigned b, unsigned inf) {
-    if ((b & 0x7FFFu) > inf) b = inf | 0x8000u;
-    if (b == 0x8000u) b = 0;
-    return b & 0x8000u ? ~b & 0xFFFFu : b | 0x8000u;
+template <> __device__ __forceinline__ unsigned key_of<__nv_bfloat16>(float l) {
+    return order16(__bfloat16_as_ushort(__float2bfloat16_rn(l)));
 }
-__device__ __forceinline__ unsigned key_of(__nv_bfloat16 l) { return key_of_bits16(__bfloat16_as_ushort(l), 0x7F80u); }
-__device__ __forceinline__ unsigned key_of(__half l) { return key_of_bits16(__half_as_ushort(l), 0x7C00u); }
+template <> __device__ __forceinline__ unsigned key_of<__half>(float l) { return order16(__half_as_ushort(__float2half_rn(l))); }
 template <class T> __device__ __forceinline__ float value_of(unsigned key);
 template <> __device__ __forceinline__ float value_of<float>(unsigned k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
@@ -440,23 +462,26 @@ struct Team {
 // A row's choices in a thread: four neighbours of each stretch of 4 TPR, so that their order is stretch, thread, place.
 template <int TPR, int EPT>
 struct RowTile {
-    unsigned key[EPT], wgt[EPT];   // 0: not legal, or cut off
+    float l[EPT];        // -inf: not legal, or cut off
+    unsigned wgt[EPT];
     __device__ static int at(int e) { return (e >> 2) * 4 * TPR + 4 * (static_cast<int>(threadIdx.x) & (TPR - 1)) + (e & 3); }
 };
 
 // Cuts the row to the shortest run of its ranked choices whose amounts (their weights, or 1 each) reach `reach` >= 1, by
-// bisection for the lowest key that stays: what lies above it does not reach. Choices of that key stay by their index.
-// n: how many choices there are; their amounts reach. guess: where to look first (0: halfway).
-template <bool WEIGHTS, int TPR, int EPT>
-__device__ __forceinline__ void cut_row(RowTile<TPR, EPT>& r, Team<TPR>& team, u64 reach, unsigned top, unsigned guess, unsigned n) {
-    unsigned lo = 0, hi = top, n_lo = n, n_hi = 0;   // amounts above lo reach, those above hi do not
-    u64 above = 0;                                   // hi's
-    unsigned mid = guess > 0 && guess < top ? guess : top / 2;
+// bisection for the lowest value that stays: what lies above it does not reach. Choices of that value stay by their index.
+// m: the largest value; n: how many there are above -inf, whose amounts reach; guess: where to look first.
+template <bool WEIGHTS, class T, int TPR, int EPT>
+__device__ __forceinline__ void cut_row(RowTile<TPR, EPT>& r, Team<TPR>& team, u64 reach, float m, float guess, unsigned n) {
+    unsigned lo = key_of<T>(-INFINITY), hi = key_of<T>(m), n_lo = n, n_hi = 0;   // amounts above lo reach, those above hi do not
+    u64 above = 0;                                                              // hi's
+    unsigned mid = key_of<T>(guess);
+    if (mid <= lo || mid >= hi) mid = lo + (hi - lo) / 2;
     while (hi - lo > 1 && n_lo - n_hi > 1) {
+        const float at = value_of<T>(mid);
         unsigned v = 0, c = 0;
 #pragma unroll
         for (int e = 0; e < EPT; ++e)
-            if (r.key[e] > mid) {
+            if (r.l[e] > at) {
                 if (WEIGHTS) v += r.wgt[e];
                 ++c;
             }
@@ -477,69 +502,72 @@ __device__ __forceinline__ void cut_row(RowTile<TPR, EPT>& r, Team<TPR>& team, u
         }
         mid = lo + (hi - lo) / 2;
     }
-    const unsigned group = n_lo - n_hi;   // all choices in (lo, hi]: one, or several of one key
-    unsigned mine = 0, low = 0, w = 0;
-#pragma unroll
-    for (int e = 0; e < EPT; ++e)
-        if (r.key[e] > lo && r.key[e] <= hi) {
-            low = r.key[e];
-            w = r.wgt[e];
-            ++mine;
-        }
-    unsigned stay = 1;
+    const float low = value_of<T>(lo), high = value_of<T>(hi);
+    const unsigned group = n_lo - n_hi;   // all choices in (low, high]: one, or several of one value
     if (group > 1) {
-        unsigned unused;
-        if (WEIGHTS) w = team.largest(w, 0, unused);
-        const u64 left = reach - above, each = WEIGHTS ? w : 1;
-        stay = each == 0 || (left + each - 1) / each >= group ? group : static_cast<unsigned>((left + each - 1) / each);
-    }
-    if (stay < group) {   // the first `stay` of the group by index
-        unsigned past = 0;
+        u64 each = 1;
+        if (WEIGHTS) {
+            unsigned w = 0, unused;
 #pragma unroll
-        for (int s = 0; s < EPT / 4; ++s) {
-            unsigned here = 0;
+            for (int e = 0; e < EPT; ++e)
+                if (r.l[e] > low && r.l[e] <= high) w = r.wgt[e];
+            each = team.largest(w, 0, unused);
+        }
+        const u64 left = reach - above, want = each == 0 ? group : (left + each - 1) / each;
+        if (want < group) {   // the first of the group by index
+            unsigned rank = 0;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) here += r.key[4 * s + q] > lo && r.key[4 * s + q] <= hi;
-            const unsigned total = team.count(here);
-            unsigned rank = past + static_cast<unsigned>(team.before(here));
+            for (int s = 0; s < EPT / 4; ++s) {
+                unsigned here = 0;
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (r.key[4 * s + q] > lo && r.key[4 * s + q] <= hi && rank++ >= stay) r.key[4 * s + q] = 0;
-            past += total;
+                for (int q = 0; q < 4; ++q) here += r.l[4 * s + q] > low && r.l[4 * s + q] <= high;
+                unsigned mine = rank + static_cast<unsigned>(team.before(here));
+                rank += team.count(here);
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (r.l[4 * s + q] > low && r.l[4 * s + q] <= high && mine++ >= want) r.l[4 * s + q] = -INFINITY;
+            }
         }
     }
 #pragma unroll
     for (int e = 0; e < EPT; ++e)
-        if (r.key[e] <= lo) r.key[e] = r.wgt[e] = 0;
+        if (!(r.l[e] > low)) {
+            r.l[e] = -INFINITY;
+            r.wgt[e] = 0;
+        }
+}
+
+// A value that at least k of the row's choices reach: k / warps of each warp's threads have a choice that reaches the warp's
+// own bound, the lowest of which holds for all. -inf where k is too large for that.
+template <class T, int TPR, int EPT>
+__device__ __forceinline__ float kth_bound(const RowTile<TPR, EPT>& r, Team<TPR>& team, unsigned k) {
+    const unsigned each = (k + Team<TPR>::kWarps - 1) / Team<TPR>::kWarps;
+    if (each > 32) return -INFINITY;
+    float best = r.l[0];
+#pragma unroll
+    for (int e = 1; e < EPT; ++e) best = fmaxf(best, r.l[e]);
+    const unsigned key = key_of<T>(best);
+    unsigned t = 0;
+    for (unsigned bit = 1u << (sizeof(T) * 8 - 1); bit; bit >>= 1) {
+        const unsigned n = __popc(__ballot_sync(~0u, key >= (t | bit)));
+        if (n >= each) t |= bit;
+        if (n == each) break;
+    }
+    unsigned unused;
+    t = ~team.largest(~t, 0, unused);
+    const unsigned floor = key_of<T>(-INFINITY);
+    return t > floor + 1 ? value_of<T>(t - 1) : -INFINITY;
 }
 
 // Warps per SM that the registers of EPT choices per thread leave room for.
 template <int EPT>
 constexpr int kRowWarps = EPT <= 4 ? 48 : EPT <= 12 ? 32 : 24;
 
-// A key that at least k of the row's choices reach, less one: k / warps of each warp's threads have a choice that reaches the
-// warp's own bound, the lowest of which holds for all. 0 where k is too large for that.
-template <int TPR, int EPT>
-__device__ __forceinline__ unsigned kth_bound(const RowTile<TPR, EPT>& r, Team<TPR>& team, unsigned k) {
-    const unsigned each = (k + Team<TPR>::kWarps - 1) / Team<TPR>::kWarps;
-    if (each > 32) return 0;
-    unsigned best = 0, t = 0;
-#pragma unroll
-    for (int e = 0; e < EPT; ++e) best = max(best, r.key[e]);
-    for (unsigned bit = 1u << (31 - __clz(__reduce_max_sync(~0u, best) | 1u)); bit; bit >>= 1) {
-        const unsigned n = __popc(__ballot_sync(~0u, best >= (t | bit)));
-        if (n >= each) t |= bit;
-        if (n == each) break;
-    }
-    unsigned unused;
-    t = ~team.largest(~t, 0, unused);
-    return t ? t - 1 : 0;
-}
-
-// A warp, or a block of TPR threads, per row; the row's keys and weights stay in registers. VEC: rows whose four
+// A warp, or a block of TPR threads, per row; the row's values and weights stay in registers. VEC: rows whose four
 // neighbours can be loaded at once.
 template <class T, int TPR, int EPT, bool VEC>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, TPR == 32 ? kRowWarps<EPT> / 8 : kRowWarps<EPT> * 32 / TPR) k_rows_sample(RowArgs a) {
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, TPR == 32 ? kRowWarps<EPT> / 8 : kRowWarps<EPT> * 32 / TPR)
+k_rows_sample(RowArgs a) {
     constexpr int kTeams = TPR == 32 ? 8 : 1;
     __shared__ u64 place[4 * Team<TPR>::kWarps];
     Team<TPR> team;
@@ -564,94 +592,101 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, TPR == 32 ? kRowWarps<E
         unsigned bits = ~0u;
         if (parts) bits = __ballot_sync(~0u, lane < kBytes && legal[min(lane, kBytes - 1)] != 0);
         RowTile<TPR, EPT> r;
-        unsigned top = 0, nans = 0;
+        float m = 0.f;
+        bool careful = false;   // a second turn: the largest legal value is not finite, or a legal one is a NaN
+        unsigned nans = 0;
+        while (true) {
+            float best = -INFINITY;
 #pragma unroll
-        for (int s = 0; s < EPT / 4; ++s) {
-            const int i = r.at(4 * s);
-            T l[4];
-            uint8_t ok[4];
-            if constexpr (VEC) {
-                if (i < n) {
-                    struct alignas(4 * sizeof(T)) Four { T v[4]; };
-                    const Four f = *reinterpret_cast<const Four*>(logits + i);
+            for (int s = 0; s < EPT / 4; ++s) {
+                const int i = r.at(4 * s);
+                float l[4];
+                bool ok[4] = {i < n, i + 1 < n, i + 2 < n, i + 3 < n};
+                if constexpr (VEC) {
+                    if (i < n) {
+                        struct alignas(4 * sizeof(T)) Four { T v[4]; };
+                        const Four f = *reinterpret_cast<const Four*>(logits + i);
 #pragma unroll
-                    for (int p = 0; p < 4; ++p) l[p] = f.v[p];
-                    if (legal && !parts) {
-                        const uchar4 m = *reinterpret_cast<const uchar4*>(legal + i);
-                        ok[0] = m.x;
-                        ok[1] = m.y;
-                        ok[2] = m.z;
-                        ok[3] = m.w;
+                        for (int p = 0; p < 4; ++p) l[p] = to_f(f.v[p]);
+                        if (legal && !parts) {
+                            const uchar4 k = *reinterpret_cast<const uchar4*>(legal + i);
+                            ok[0] = k.x;
+                            ok[1] = k.y;
+                            ok[2] = k.z;
+                            ok[3] = k.w;
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int p = 0; p < 4; ++p)
+                        if (i + p < n) {
+                            l[p] = to_f(logits[i + p]);
+                            if (legal && !parts) ok[p] = legal[i + p];
+                        }
+                }
+                if constexpr (TPR == 32 && EPT == 12) {
+                    if (parts && i < n) {
+                        const uint4 v = need_s[i >> 2];
+                        ok[0] = (bits & v.x) == v.x;
+                        ok[1] = (bits & v.y) == v.y;
+                        ok[2] = (bits & v.z) == v.z;
+                        ok[3] = (bits & v.w) == v.w;
                     }
                 }
-            } else {
 #pragma unroll
-                for (int p = 0; p < 4; ++p)
-                    if (i + p < n) {
-                        l[p] = logits[i + p];
-                        if (legal && !parts) ok[p] = legal[i + p];
+                for (int p = 0; p < 4; ++p) {
+                    float v = ok[p] ? l[p] : -INFINITY;
+                    if (careful) {   // m: the largest that is no NaN; what equals it becomes 0 if it is not finite
+                        if (fabsf(m) < INFINITY) v = v == v ? v : -INFINITY;
+                        else v = ok[p] && (m < 0.f ? !(v > m) : v == m) ? 0.f : -INFINITY;
                     }
-            }
-            unsigned need[4] = {0, 0, 0, 0};
-            if constexpr (TPR == 32 && EPT == 12) {
-                if (parts && i < n) {
-                    const uint4 v = need_s[i >> 2];
-                    need[0] = v.x;
-                    need[1] = v.y;
-                    need[2] = v.z;
-                    need[3] = v.w;
+                    r.l[4 * s + p] = v;
+                    best = max_nan(best, v);
                 }
             }
+            const bool bad = best != best;
+            if (bad) {
+                best = -INFINITY;
 #pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                const int e = 4 * s + p;
-                bool in = i + p < n && (bits & need[p]) == need[p];
-                if (legal && !parts) in = in && ok[p] != 0;
-                r.key[e] = in ? key_of(l[p]) : 0u;
-                nans |= in && to_f(l[p]) != to_f(l[p]);
-                top = max(top, r.key[e]);
+                for (int e = 0; e < EPT; ++e) best = fmaxf(best, r.l[e]);
             }
+            unsigned found;
+            m = value_of<float>(team.largest(key_of<float>(best), bad, found));
+            if (careful || (found == 0 && fabsf(m) < INFINITY)) break;
+            nans = found;
+            careful = true;
         }
-        top = team.largest(top, nans, nans);
-        if (top == 0) {   // nothing legal
+        if (m == -INFINITY) {   // nothing legal
             if ((threadIdx.x & (TPR - 1)) == 0) {
                 a.choice[row] = 0;
                 a.logp[row] = 0.f;
             }
             continue;
         }
-        const float m = value_of<T>(top);
-        unsigned mine = 0;   // legal choices
 #pragma unroll
-        for (int e = 0; e < EPT; ++e) {
-            const float l = value_of<T>(r.key[e]);
-            r.wgt[e] = r.key[e] ? weight_of(l == m ? 0.f : (l - m) * q.scale) : 0u;
-            mine += r.key[e] != 0;
-        }
+        for (int e = 0; e < EPT; ++e) r.wgt[e] = weight_of((r.l[e] - m) * q.scale);
         if (q.top_k > 0) {
-            const unsigned k = static_cast<unsigned>(q.top_k), count = team.count(mine);
-            if (k < count) cut_row<false>(r, team, k, top, kth_bound(r, team, k), count);
+            unsigned count = 0;
+#pragma unroll
+            for (int e = 0; e < EPT; ++e) count += r.l[e] > -INFINITY;
+            count = team.count(count);
+            const unsigned k = static_cast<unsigned>(q.top_k);
+            if (k < count) cut_row<false, T>(r, team, k, m, kth_bound<T>(r, team, k), count);
         }
         if (q.top_p < 1.f) {
             unsigned w = 0, count = 0;
 #pragma unroll
             for (int e = 0; e < EPT; ++e) {
-                if (!r.wgt[e]) r.key[e] = 0;   // a choice that weighs nothing adds nothing
                 w += r.wgt[e];
-                count += r.key[e] != 0;
+                count += r.l[e] > -INFINITY;
             }
             u64 total;
             team.sums(w, count, total, count);
             const double p = ceil(static_cast<double>(q.top_p) * static_cast<double>(total));
             const u64 reach = p < 1.0 ? 1ull : static_cast<u64>(p);
-            // choices that could all go together are below the lowest key that stays: look at the best of them first
-            const float least = static_cast<float>(total - reach) / static_cast<float>(count);
-            unsigned guess = 0, unused;
-#pragma unroll
-            for (int e = 0; e < EPT; ++e)
-                if (static_cast<float>(r.wgt[e]) <= least) guess = max(guess, r.key[e]);
-            guess = team.largest(guess, 0, unused);
-            cut_row<true>(r, team, reach, top, guess, count);
+            // choices that could all go together lie below the lowest value that stays: look there first
+            const float least = static_cast<float>(total - reach) * kUnit / static_cast<float>(count);
+            cut_row<true, T>(r, team, reach, m, m + __logf(least) / q.scale, count);
         }
         if (q.min_p > 0.f) {
             const unsigned least = static_cast<unsigned>(ceil(static_cast<double>(q.min_p) * static_cast<double>(kScale)));
@@ -668,7 +703,8 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, TPR == 32 ? kRowWarps<E
         }
         u64 target = (bits24(u) * total) >> 24;
         int stretch = 0;
-        unsigned w[4] = {r.wgt[0], r.wgt[1], r.wgt[2], r.wgt[3]}, k[4] = {r.key[0], r.key[1], r.key[2], r.key[3]};
+        unsigned w[4] = {r.wgt[0], r.wgt[1], r.wgt[2], r.wgt[3]};
+        float l[4] = {r.l[0], r.l[1], r.l[2], r.l[3]};
 #pragma unroll
         for (int s = 1; s < EPT / 4; ++s)
             if (stretch == s - 1 && target >= part[s - 1]) {
@@ -677,25 +713,23 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, TPR == 32 ? kRowWarps<E
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
                     w[p] = r.wgt[4 * s + p];
-                    k[p] = r.key[4 * s + p];
+                    l[p] = r.l[4 * s + p];
                 }
             }
         const u64 own = static_cast<u64>(w[0]) + w[1] + w[2] + w[3], run = team.before(own);
         if (run <= target && target < run + own) {
             unsigned left = static_cast<unsigned>(target - run);
             int c = 0;
-            unsigned key = k[0];
+            float lc = l[0];
 #pragma unroll
             for (int p = 0; p < 3; ++p)
                 if (c == p && left >= w[p]) {
                     left -= w[p];
                     c = p + 1;
-                    key = k[p + 1];
+                    lc = l[p + 1];
                 }
-            const float l = value_of<T>(key);
-            const float lp = (l == m ? 0.f : (l - m) * q.scale) - logf(static_cast<float>(total) * kUnit);
             a.choice[row] = r.at(4 * stretch) + c;
-            a.logp[row] = nans ? NAN : lp;
+            a.logp[row] = nans ? NAN : (lc - m) * q.scale - logf(static_cast<float>(total) * kUnit);
         }
     }
 }
@@ -734,50 +768,57 @@ __device__ __forceinline__ void fetch_batch(const LogpArgs& a, long long first, 
     copies_commit();
 }
 
-// A part's softmax over its legal choices: l - m, exp(l - m), their sum, and sum w (l - m) / S: log p = d - log S and the
-// entropy is log S - mean_d, so log p + H = d - mean_d needs no logarithm.
+// A part's softmax over its legal choices: d = l - m (-200 where that is lower: such weights are 0 either way), w = exp(d),
+// 1 / S, and mean_d = sum w d / S: log p = d - log S and the entropy is log S - mean_d, so log p + H = d - mean_d needs no
+// logarithm. exp as 2^(d log2 e) by the hardware's instruction, 2 ulp: the rounding of d itself costs as much.
 template <int N>
 struct Soft {
     float d[N], w[N], sum, inv, mean_d;
-    unsigned legal;
+    float choice_d;   // the choice's d; -inf where it is not legal
 };
 
+// False where nothing is legal.
 template <int K, class T>
-__device__ __forceinline__ void soft_part(Soft<part_n(K)>& s, const T* logits, const uint8_t* mask, const float* tab,
+__device__ __forceinline__ bool soft_part(Soft<part_n(K)>& s, const T* logits, const uint8_t* mask, const float* tab,
                                           const int* c) {
     constexpr int N = part_n(K);
-    part_logits<K>(s.d, logits, tab, c);
-    s.legal = part_legal<K>(mask);
-    float m = -INFINITY;
+    part_logits<K>(s.d, logits, mask, tab, c);
+    float m = s.d[0];
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-        if (s.legal >> i & 1) m = fmaxf(m, s.d[i]);
+    for (int i = 1; i < N; ++i) m = max_nan(m, s.d[i]);
+    bool some = true;
+    if (fabsf(m) == INFINITY) {
+        float v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = s.d[i];
+        some = settle<N>(v, mask + part_at(K), m);
+#pragma unroll
+        for (int i = 0; i < N; ++i) s.d[i] = v[i];
+    }
     s.sum = 0.f;
+    s.choice_d = 0.f;
     float t = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        s.d[i] = s.d[i] == m ? 0.f : s.d[i] - m;
-        s.w[i] = s.legal >> i & 1 ? expf(s.d[i]) : 0.f;
+        const float d = s.d[i] - m;
+        if (i == c[K]) s.choice_d = d;
+        s.d[i] = max_nan(d, -200.f);
+        s.w[i] = __expf(s.d[i]);
         s.sum += s.w[i];
-        if (s.w[i] != 0.f) t = fmaf(s.w[i], s.d[i], t);
+        t = fmaf(s.w[i], s.d[i], t);
     }
     s.inv = __frcp_rn(s.sum);
     s.mean_d = t * s.inv;
+    return some;
 }
 
 // Adds the choice's d, and mean_d, and multiplies the sum in: one logarithm for the five parts.
 template <int K, class T>
 __device__ __forceinline__ void logp_part(const T* logits, const uint8_t* mask, const float* tab, const int* c, float& d_sum,
                                           float& mean_sum, float& sums) {
-    constexpr int N = part_n(K);
-    Soft<N> s;
-    soft_part<K>(s, logits, mask, tab, c);
-    if (!s.legal) return;
-    float dc = -INFINITY;   // a choice that is not legal
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-        if (i == c[K] && (s.legal >> i & 1)) dc = s.d[i];
-    d_sum += dc;
+    Soft<part_n(K)> s;
+    if (!soft_part<K>(s, logits, mask, tab, c)) return;
+    d_sum += s.choice_d;
     mean_sum += s.mean_d;
     sums *= s.sum;
 }
@@ -835,14 +876,14 @@ __device__ __forceinline__ void grad_part(T* logits, const uint8_t* mask, const 
                                           float* acc) {
     constexpr int N = part_n(K);
     Soft<N> s;
-    soft_part<K>(s, logits, mask, tab, c);
+    const bool some = soft_part<K>(s, logits, mask, tab, c);
+    const int hit = some && mask[part_at(K) + c[K]] != 0 ? c[K] : -1;
+    if (!some) ga = gb = s.inv = s.mean_d = 0.f;
     float g[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const float p = s.w[i] * s.inv;
-        g[i] = i == c[K] ? ga : 0.f;
-        if (p != 0.f) g[i] = fmaf(-p, fmaf(gb, s.d[i] - s.mean_d, ga), g[i]);
-        if (!(s.legal >> i & 1)) g[i] = 0.f;
+        g[i] = fmaf(-p, fmaf(gb, s.d[i] - s.mean_d, ga), i == hit ? ga : 0.f);
     }
     if constexpr (K > 0) {
         if (acc) {

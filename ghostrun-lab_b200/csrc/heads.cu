@@ -163,20 +163,19 @@ __device__ __forceinline__ void stage(T* dst, const void* base, long long first,
 
 // Logits of a part whose largest legal one is not finite, brought to the case where it is: what equals it (or, for -inf, what
 // is legal at all) becomes 0, the rest -inf. A NaN is taken as -inf. False where nothing is legal.
-template <int N>
-__device__ __noinline__ bool settle(float* l, const uint8_t* mask, float& m) {
+__device__ __noinline__ bool settle(float* l, int n, const uint8_t* mask, float& m) {
     m = -INFINITY;
     bool any = false;
-    for (int i = 0; i < N; ++i) {
+    for (int i = 0; i < n; ++i) {
         m = fmaxf(m, l[i]);
         any |= mask[i] != 0;
     }
     if (fabsf(m) < INFINITY) {   // there was a NaN
-        for (int i = 0; i < N; ++i)
+        for (int i = 0; i < n; ++i)
             if (l[i] != l[i]) l[i] = -INFINITY;
         return any;
     }
-    for (int i = 0; i < N; ++i) l[i] = mask[i] != 0 && (m < 0.f ? !(l[i] > m) : l[i] == m) ? 0.f : -INFINITY;
+    for (int i = 0; i < n; ++i) l[i] = mask[i] != 0 && (m < 0.f ? !(l[i] > m) : l[i] == m) ? 0.f : -INFINITY;
     m = 0.f;
     return any;
 }
@@ -194,7 +193,7 @@ __device__ __forceinline__ int choose(float (&l)[N], const uint8_t* mask, float 
         float v[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = l[i];
-        if (!settle<N>(v, mask, m)) return 0;
+        if (!settle(v, N, mask, m)) return 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) l[i] = v[i];
     }
@@ -790,75 +789,84 @@ struct LogpArgs {
     long long rows;
 };
 
-template <class T, int ROWS>
+template <class T>
 struct LogpBatch {
-    T logits[ROWS * kBytes];
-    alignas(16) uint8_t masks[ROWS * kBytes];
+    T logits[kThreads * kBytes];
+    alignas(16) uint8_t masks[kThreads * kBytes];
 };
 
-template <class T, int ROWS>
-__device__ __forceinline__ void fetch_batch(const LogpArgs& a, long long first, LogpBatch<T, ROWS>& to) {
+template <class T>
+__device__ __forceinline__ void fetch_batch(const LogpArgs& a, long long first, LogpBatch<T>& to) {
     if (first < a.rows) {
-        const int n = static_cast<int>(min(static_cast<long long>(ROWS), a.rows - first));
+        const int n = static_cast<int>(min(static_cast<long long>(kThreads), a.rows - first));
         stage<kBytes>(to.logits, a.logits, first, n, a.stride, a.dense_logits);
         stage<kBytes>(to.masks, a.masks, first, n, a.mask_stride, a.dense_masks);
     }
     copies_commit();
 }
 
-// A part's softmax over its legal choices: d = l - m (-200 where that is lower: such weights are 0 either way), w = exp(d),
-// 1 / S, and mean_d = sum w d / S: log p = d - log S and the entropy is log S - mean_d, so log p + H = d - mean_d needs no
-// logarithm. exp as 2^(d log2 e) by the hardware's instruction, 2 ulp: the rounding of d itself costs as much.
-template <int N>
-struct Soft {
-    float d[N], w[N], sum, inv, mean_d;
-    float choice_d;   // the choice's d; -inf where it is not legal
+// The five parts' softmaxes over their legal choices: d = l - m (-200 where that is lower: such weights are 0 either way),
+// w = exp(d), S = sum w, 1 / S, and mean_d = sum w d / S: log p = d - log S and the entropy is log S - mean_d, so log p + H =
+// d - mean_d needs no logarithm. exp as 2^(d log2 e) by the hardware's instruction, 2 ulp: the rounding of d itself costs as
+// much. The choices are known, so the parts do not wait for one another: all 19 logits go side by side.
+struct SoftRow {
+    float d[kBytes], w[kBytes], sum[kParts], inv[kParts], mean_d[kParts];
+    float choice_d[kParts];   // the choice's d; -inf where it is not legal
+    unsigned some;            // bit k: part k has a legal choice
 };
 
-// False where nothing is legal.
-template <int K, class T>
-__device__ __forceinline__ bool soft_part(Soft<part_n(K)>& s, const T* logits, const uint8_t* mask, const float* tab,
-                                          const int* c) {
-    constexpr int N = part_n(K);
-    part_logits<K>(s.d, logits, mask, tab, c);
-    float m = s.d[0];
+template <class T>
+__device__ __forceinline__ void soft_row(SoftRow& s, const T* logits, const uint8_t* mask, const float* tab, const int* c) {
 #pragma unroll
-    for (int i = 1; i < N; ++i) m = max_nan(m, s.d[i]);
-    bool some = true;
-    if (fabsf(m) == INFINITY) {
-        float v[N];
+    for (int k = 0; k < kParts; ++k)
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = s.d[i];
-        some = settle<N>(v, mask + part_at(K), m);
+        for (int i = 0; i < part_n(k); ++i) {
+            const int e = part_at(k) + i;
+            float l = to_f(logits[e]);
+            if (tab) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) s.d[i] = v[i];
+                for (int j = 0; j < k; ++j) l += tab[table_at(table_of(k, j)) + c[j] * part_n(k) + i];
+            }
+            s.d[e] = mask[e] != 0 ? l : -INFINITY;
+        }
+    float m[kParts];
+    bool odd = false;
+#pragma unroll
+    for (int k = 0; k < kParts; ++k) {
+        m[k] = s.d[part_at(k)];
+#pragma unroll
+        for (int i = 1; i < part_n(k); ++i) m[k] = max_nan(m[k], s.d[part_at(k) + i]);
+        odd |= fabsf(m[k]) == INFINITY;
     }
-    s.sum = 0.f;
-    s.choice_d = 0.f;
-    float t = 0.f;
+    s.some = 31;
+    if (odd) {
+        float v[kBytes];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const float d = s.d[i] - m;
-        if (i == c[K]) s.choice_d = d;
-        s.d[i] = max_nan(d, -200.f);
-        s.w[i] = __expf(s.d[i]);
-        s.sum += s.w[i];
-        t = fmaf(s.w[i], s.d[i], t);
+        for (int e = 0; e < kBytes; ++e) v[e] = s.d[e];
+#pragma unroll
+        for (int k = 0; k < kParts; ++k)
+            if (fabsf(m[k]) == INFINITY && !settle(v + part_at(k), part_n(k), mask + part_at(k), m[k])) s.some &= ~(1u << k);
+#pragma unroll
+        for (int e = 0; e < kBytes; ++e) s.d[e] = v[e];
     }
-    s.inv = __fdividef(1.f, s.sum);   // the hardware's reciprocal, 1 ulp; S is between 1 and 9
-    s.mean_d = t * s.inv;
-    return some;
-}
-
-// Adds the choice's d, and mean_d, and multiplies the sum in: one logarithm for the five parts.
-template <int K, class T>
-__device__ __forceinline__ void logp_part(const T* logits, const uint8_t* mask, const float* tab, const int* c, float& d_sum,
-                                          float& mean_sum, float& sums) {
-    Soft<part_n(K)> s;
-    if (!soft_part<K>(s, logits, mask, tab, c)) return;
-    d_sum += s.choice_d;
-    mean_sum += s.mean_d;
-    sums *= s.sum;
+#pragma unroll
+    for (int k = 0; k < kParts; ++k) {
+        float sum = 0.f, t = 0.f;
+        s.choice_d[k] = 0.f;
+#pragma unroll
+        for (int i = 0; i < part_n(k); ++i) {
+            const int e = part_at(k) + i;
+            const float d = s.d[e] - m[k];
+            if (i == c[k]) s.choice_d[k] = d;
+            s.d[e] = max_nan(d, -200.f);
+            s.w[e] = __expf(s.d[e]);
+            sum += s.w[e];
+            t = fmaf(s.w[e], s.d[e], t);
+        }
+        s.sum[k] = sum;
+        s.inv[k] = __fdividef(1.f, sum);   // the hardware's reciprocal, 1 ulp; S is between 1 and 9
+        s.mean_d[k] = t * s.inv[k];
+    }
 }
 
 __device__ __forceinline__ bool parts_of(int id, int* c) {
@@ -876,7 +884,7 @@ template <class T>
 __global__ void __launch_bounds__(kThreads) k_moves_logp(LogpArgs a) {
     extern __shared__ __align__(16) unsigned char batches[];
     __shared__ float tab_s[kCond];
-    auto* batch = reinterpret_cast<LogpBatch<T, kThreads>*>(batches);
+    auto* batch = reinterpret_cast<LogpBatch<T>*>(batches);
     const long long step = static_cast<long long>(gridDim.x) * kThreads;
     long long first = static_cast<long long>(blockIdx.x) * kThreads;
     fetch_batch(a, first, batch[0]);
@@ -893,12 +901,16 @@ __global__ void __launch_bounds__(kThreads) k_moves_logp(LogpArgs a) {
             const bool known = parts_of(id, c);   // else no move has this id
             const T* logits = batch[b].logits + threadIdx.x * kBytes;
             const uint8_t* mask = batch[b].masks + threadIdx.x * kBytes;
-            float d_sum = 0.f, mean_sum = 0.f, sums = 1.f;
-            logp_part<0>(logits, mask, tab, c, d_sum, mean_sum, sums);
-            logp_part<1>(logits, mask, tab, c, d_sum, mean_sum, sums);
-            logp_part<2>(logits, mask, tab, c, d_sum, mean_sum, sums);
-            logp_part<3>(logits, mask, tab, c, d_sum, mean_sum, sums);
-            logp_part<4>(logits, mask, tab, c, d_sum, mean_sum, sums);
+            SoftRow s;
+            soft_row(s, logits, mask, tab, c);
+            float d_sum = 0.f, mean_sum = 0.f, sums = 1.f;   // one logarithm for the five parts
+#pragma unroll
+            for (int k = 0; k < kParts; ++k)
+                if (s.some >> k & 1) {
+                    d_sum += s.choice_d[k];
+                    mean_sum += s.mean_d[k];
+                    sums *= s.sum[k];
+                }
             const float log_sums = logf(sums);
             a.logp[row] = known ? d_sum - log_sums : NAN;
             a.entropy[row] = known ? log_sums - mean_sum : NAN;
@@ -907,111 +919,88 @@ __global__ void __launch_bounds__(kThreads) k_moves_logp(LogpArgs a) {
     }
 }
 
-// A row of the backward: its place in the batch, its choices (part 0 first) and incoming gradients.
-template <class T>
-struct GradRow {
-    T* logits;
-    const uint8_t* mask;
-    int c[kParts];
-    float ga, gb;
-};
-
-// dl = ga 1[i = c] - p (ga + gb (d - mean_d)) of part K of two rows, in the logits' place; acc: this thread's own column of
-// the block's table sums, kThreads apart (no two of the additions of a row's part go to one place, so they are read and
-// written together).
-template <int K, class T>
-__device__ __forceinline__ void grad_part(GradRow<T> (&row)[2], const float* tab, float* acc) {
-    constexpr int N = part_n(K);
-    float g[2][N];
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        const GradRow<T>& r = row[q];
-        Soft<N> s;
-        const bool some = soft_part<K>(s, r.logits, r.mask, tab, r.c);
-        const int hit = some && r.mask[part_at(K) + r.c[K]] != 0 ? r.c[K] : -1;
-        const float ga = some ? r.ga : 0.f, gb = some ? r.gb : 0.f;
-        if (!some) s.inv = s.mean_d = 0.f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float p = s.w[i] * s.inv;
-            g[q][i] = fmaf(-p, fmaf(gb, s.d[i] - s.mean_d, ga), i == hit ? ga : 0.f);
-        }
-    }
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        if constexpr (K > 0) {
-            if (acc) {
-                float sum[K * N];
-#pragma unroll
-                for (int j = 0; j < K; ++j)
-#pragma unroll
-                    for (int i = 0; i < N; ++i)
-                        sum[j * N + i] = acc[(table_at(table_of(K, j)) + row[q].c[j] * N + i) * kThreads] + g[q][i];
-#pragma unroll
-                for (int j = 0; j < K; ++j)
-#pragma unroll
-                    for (int i = 0; i < N; ++i)
-                        acc[(table_at(table_of(K, j)) + row[q].c[j] * N + i) * kThreads] = sum[j * N + i];
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) row[q].logits[part_at(K) + i] = from_f<T>(g[q][i]);
-    }
-}
-
-// Two rows per thread at a time (the table sums leave room for 8 warps per SM: two independent rows each hide their
-// latency; 89 us for 8,192 x 128 rows with one). Every thread sums the tables' gradient in a column of its own of shared
-// memory, so that no two add to one place and the order of the additions is the launch's alone.
+// A thread per row: dl = ga 1[i = c] - p (ga + gb (d - mean_d)), in the logits' place in shared memory and from there to
+// memory as one stretch. Every thread sums the tables' gradient in a column of its own of shared memory (65 KB per block,
+// which leaves 8 warps per SM), so that no two add to one place and the order of the additions is the launch's alone; the
+// 23 additions of a row go to 23 places, so they are read together and written together.
 template <class T>
 __global__ void __launch_bounds__(kThreads) k_moves_grad(LogpArgs a) {
-    extern __shared__ __align__(16) unsigned char batches[];   // a batch, then [127][kThreads] sums
+    extern __shared__ __align__(16) unsigned char batches[];   // two batches, then [127][kThreads] sums
     __shared__ float tab_s[kCond];
     __shared__ uint8_t none_s[kBytes];
-    constexpr int kRows = 2 * kThreads;
-    auto& batch = *reinterpret_cast<LogpBatch<T, kRows>*>(batches);
-    float* acc_s = reinterpret_cast<float*>(batches + sizeof(batch));
-    const long long step = static_cast<long long>(gridDim.x) * kRows;
+    auto* batch = reinterpret_cast<LogpBatch<T>*>(batches);
+    float* acc_s = reinterpret_cast<float*>(batches + 2 * sizeof(LogpBatch<T>));
+    const long long step = static_cast<long long>(gridDim.x) * kThreads;
+    long long first = static_cast<long long>(blockIdx.x) * kThreads;
+    fetch_batch(a, first, batch[0]);
     if (threadIdx.x < kBytes) none_s[threadIdx.x] = 0;
     load_cond(tab_s, a.cond);
     float* acc = a.part ? acc_s + threadIdx.x : nullptr;
     if (acc)
         for (int e = 0; e < kCond; ++e) acc[e * kThreads] = 0.f;
     const float* tab = a.cond.type < 0 ? nullptr : tab_s;
-    for (long long first = static_cast<long long>(blockIdx.x) * kRows; first < a.rows; first += step) {
-        fetch_batch(a, first, batch);
-        GradRow<T> row[2];
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const int at = threadIdx.x + q * kThreads;
-            const long long i = first + at;
-            row[q].logits = batch.logits + at * kBytes;
-            row[q].mask = batch.masks + at * kBytes;
-            row[q].ga = row[q].gb = 0.f;
-            int id = -1;
-            if (i < a.rows) {
-                id = a.ids[i];
-                if (a.glp) row[q].ga = a.glp[i * a.glp_stride];
-                if (a.gent) row[q].gb = a.gent[i * a.gent_stride];
-            }
-            // behind the last row, or an id that no move has: nothing is legal, so nothing is added
-            if (!parts_of(id, row[q].c)) row[q].mask = none_s;
+    for (int b = 0; first < a.rows; first += step, b ^= 1) {
+        fetch_batch(a, first + step, batch[b ^ 1]);
+        const long long row = first + threadIdx.x;
+        float ga = 0.f, gb = 0.f;
+        int id = -1, c[kParts];
+        if (row < a.rows) {
+            id = a.ids[row];
+            if (a.glp) ga = a.glp[row * a.glp_stride];
+            if (a.gent) gb = a.gent[row * a.gent_stride];
         }
-        copies_wait<0>();
+        copies_wait<1>();
         __syncthreads();
-        grad_part<0>(row, tab, acc);
-        grad_part<1>(row, tab, acc);
-        grad_part<2>(row, tab, acc);
-        grad_part<3>(row, tab, acc);
-        grad_part<4>(row, tab, acc);
+        T* logits = batch[b].logits + threadIdx.x * kBytes;
+        const uint8_t* mask = batch[b].masks + threadIdx.x * kBytes;
+        if (!parts_of(id, c)) mask = none_s;   // behind the last row, or no move's id: nothing is legal, nothing is added
+        {
+            SoftRow s;
+            soft_row(s, logits, mask, tab, c);
+            float g[kBytes];
+#pragma unroll
+            for (int k = 0; k < kParts; ++k) {
+                const bool some = s.some >> k & 1;
+                const int hit = some && mask[part_at(k) + c[k]] != 0 ? c[k] : -1;
+                const float gk = some ? ga : 0.f, bk = some ? gb : 0.f, inv = some ? s.inv[k] : 0.f;
+                const float mean = some ? s.mean_d[k] : 0.f;
+#pragma unroll
+                for (int i = 0; i < part_n(k); ++i) {
+                    const int e = part_at(k) + i;
+                    g[e] = fmaf(-s.w[e] * inv, fmaf(bk, s.d[e] - mean, gk), i == hit ? gk : 0.f);
+                }
+            }
+            if (acc) {
+                float sum[23];
+                int n = 0;
+#pragma unroll
+                for (int k = 1; k < kParts; ++k)
+#pragma unroll
+                    for (int j = 0; j < k; ++j)
+#pragma unroll
+                        for (int i = 0; i < part_n(k); ++i)
+                            sum[n++] = acc[(table_at(table_of(k, j)) + c[j] * part_n(k) + i) * kThreads] + g[part_at(k) + i];
+                n = 0;
+#pragma unroll
+                for (int k = 1; k < kParts; ++k)
+#pragma unroll
+                    for (int j = 0; j < k; ++j)
+#pragma unroll
+                        for (int i = 0; i < part_n(k); ++i)
+                            acc[(table_at(table_of(k, j)) + c[j] * part_n(k) + i) * kThreads] = sum[n++];
+            }
+#pragma unroll
+            for (int e = 0; e < kBytes; ++e) logits[e] = from_f<T>(g[e]);
+        }
         __syncthreads();
         if (a.dlogits) {
-            const int n = static_cast<int>(min(static_cast<long long>(kRows), a.rows - first)) * kBytes;
+            const int n = static_cast<int>(min(static_cast<long long>(kThreads), a.rows - first)) * kBytes;
             T* out = static_cast<T*>(a.dlogits) + first * kBytes;
             constexpr int kPer = 16 / static_cast<int>(sizeof(T));
             const int whole = a.dense_out ? n & ~(kPer - 1) : 0;
             for (int i = threadIdx.x * kPer; i < whole; i += kThreads * kPer)
-                *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<const uint4*>(batch.logits + i);
-            for (int i = whole + threadIdx.x; i < n; i += kThreads) out[i] = batch.logits[i];
+                *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<const uint4*>(batch[b].logits + i);
+            for (int i = whole + threadIdx.x; i < n; i += kThreads) out[i] = batch[b].logits[i];
         }
         __syncthreads();   // the batch may be written again
     }
@@ -1222,7 +1211,7 @@ int rl_moves_logp(const void* logits, long long stride, int type, const void* co
     const unsigned grid = blocks_for(rows, kThreads, 8ll * sm_count());
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        k_moves_logp<T><<<grid, kThreads, 2 * sizeof(LogpBatch<T, kThreads>), static_cast<cudaStream_t>(stream)>>>(a);
+        k_moves_logp<T><<<grid, kThreads, 2 * sizeof(LogpBatch<T>), static_cast<cudaStream_t>(stream)>>>(a);
     });
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? 0 : failed(cudaGetErrorString(e));
@@ -1257,12 +1246,12 @@ int rl_moves_logp_bwd(const void* glp, long long glp_stride, const void* gent, l
     a.dense_logits = dense(logits, stride == kBytes);
     a.dense_masks = dense(masks, mask_stride == kBytes);
     a.dense_out = dense(dlogits, true);
-    const unsigned grid = blocks_for(rows, 2 * kThreads, static_cast<long long>(kGradBlocks) * sm_count());
+    const unsigned grid = blocks_for(rows, kThreads, static_cast<long long>(kGradBlocks) * sm_count());
     auto s = static_cast<cudaStream_t>(stream);
     cudaError_t e = cudaSuccess;
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        e = launch<k_moves_grad<T>>(grid, sizeof(LogpBatch<T, 2 * kThreads>) + (dcond ? kGradSums : 0), s, a);
+        e = launch<k_moves_grad<T>>(grid, 2 * sizeof(LogpBatch<T>) + (dcond ? kGradSums : 0), s, a);
     });
     if (e == cudaSuccess) e = cudaGetLastError();
     if (e == cudaSuccess && dcond) {

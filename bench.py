@@ -69,6 +69,8 @@ def parse():
                          'policy input stem (colour lookup + 2x2 conv, tcgen05) on packed pictures; learner: '
                          'minibatches of rollout rows gathered from a pinned host region and unpacked')
     ap.add_argument('--units', type=int, default=4, help='config5: parts of the envs, each on its own stream')
+    ap.add_argument('--fused-policy', action='store_true',
+                    help="config5: the policy's layer norms and move sampling on this library's kernels")
     ap.add_argument('--seed', type=int, default=1)
     ap.add_argument('--age', type=int, default=1024,
                     help='untimed decisions before the warm-up, so that episode restarts run at their steady-state rate')
@@ -565,7 +567,7 @@ def config5_arm(args):
         env.step()
     torch.manual_seed(args.seed)
     palette = torch.rand(512, 3, generator=torch.Generator().manual_seed(args.seed))   # a seeded stand-in colour table
-    pol = Policy(palette).to(dev).to(memory_format=torch.channels_last).eval()
+    pol = Policy(palette, fused=args.fused_policy).to(dev).to(memory_format=torch.channels_last).eval()
     n_params = sum(p.numel() for p in pol.parameters())
     cuts = [E * j // U for j in range(U + 1)]
     units = [slice(cuts[j], cuts[j + 1]) for j in range(U)]
@@ -670,7 +672,8 @@ def config5_arm(args):
             ms_per_step=round(ms / K, 4), higher_is_better=True, scaling='weak', vs_baseline=None, dtype='u8+bf16',
             data='synthetic (seeded NROM cart synth00; random-init policy, seeded stand-in palette)',
             config=dict(workload=f'config 5: config 2 cart, {E} envs/GPU + the reference policy network '
-                                 f'({n_params} parameters, bf16) choosing every move, {U} parts on their own streams',
+                                 f'({n_params} parameters, bf16) choosing every move, {U} parts on their own streams'
+                                 + (', norms and move sampling fused' if args.fused_policy else ''),
                         envs_per_gpu=E, units=U, policy_parameters=n_params, frames_per_decision=4,
                         parallelism=f'dp{world} (env + policy shards)', aged_decisions=args.age,
                         inputs_exceed_l2=True),
@@ -687,7 +690,8 @@ def config5_arm(args):
                           peak_source=f'{peak_kind} (MEASURED_PEAKS.json hbm_gbs)' if peak_kind == 'measured' else 'fallback',
                           render_ms_per_decision=round(render_ms, 4)),
             kernel_ms_per_step={k: round(v / K, 4) for k, v in tm['ms'].items()},
-            gpu_launches=tm['total_launches'] + K * U,   # env kernels + one stem launch per part and decision
+            # env kernels + one stem launch per part and decision (fused: and three norms and one draw)
+            gpu_launches=tm['total_launches'] + K * U * (5 if args.fused_policy else 1),
             clocks=clk.summary(), episodes_ended=int(tot.item()), cpu_baseline=None)
     if world > 1:
         dist.barrier()

@@ -39,6 +39,25 @@ __device__ __forceinline__ float load_param(const void* p, int type, long long i
     if (type == 1) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
     return __half2float(static_cast<const __half*>(p)[i]);
 }
+// N neighbouring elements from i on (0 behind `width`), 16 bytes at a time where `wide` says that they start there.
+template <int N>
+__device__ __forceinline__ void load_params(float* out, const void* p, int type, int i, int width, bool wide, float missing) {
+    if (p && N > 1 && wide && i < width) {   // whole vectors: the width is a multiple of N
+        if (type == 0) {
+#pragma unroll
+            for (int q = 0; q < N / 4; ++q) {
+                const float4 v = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i)[q];
+                out[4 * q] = v.x;
+                out[4 * q + 1] = v.y;
+                out[4 * q + 2] = v.z;
+                out[4 * q + 3] = v.w;
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < N; ++q) out[q] = p && i + q < width ? load_param(p, type, i + q) : missing;
+}
 __device__ __forceinline__ void store_param(void* p, int type, long long i, float v) {
     if (type == 0) static_cast<float*>(p)[i] = v;
     else if (type == 1) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
@@ -51,6 +70,7 @@ struct FwdArgs {
     float2* stats;   // mean and 1 / sqrt(v + eps) of each row, or null
     long long rows, width, x_stride, r_stride;
     int w_type;
+    bool w_wide;     // weight and bias start at 16 bytes
     float eps;
 };
 
@@ -61,6 +81,7 @@ struct BwdArgs {
     float* part;     // [splits][2][width]
     long long rows, width, gy_stride, gsum_stride, s_stride;
     int w_type;
+    bool w_wide;
     int splits;
 };
 
@@ -184,7 +205,7 @@ struct Bwd : Tile<TX, VEC, TPR, EPT> {
     static constexpr int kW = kWords<TX, VEC, EPT>, kG = kWords<TY, VEC, EPT>;
     static constexpr int kDepth = depth_of<2 * kW + kG>(kBwdWarps);
     static constexpr size_t kRing = static_cast<size_t>(kDepth) * (2 * kW + kG) * 16 * Bwd::kBlock;
-    static constexpr size_t kCols = 2 * sizeof(float) * TPR * EPT;   // at the end, in the ring's place
+    static constexpr size_t kCols = 2 * sizeof(float) * EPT * Bwd::kBlock;   // at the end, in the ring's place
     static constexpr size_t kSmem = kRing > kCols ? kRing : kCols;
 };
 
@@ -198,15 +219,6 @@ k_norm_fwd(FwdArgs a) {
     __shared__ float red[2][B / 32];
     const int t = threadIdx.x % TPR, width = static_cast<int>(a.width);
     const float inv = 1.f / static_cast<float>(width);
-    float w[EPT], b[EPT];
-#pragma unroll
-    for (int v = 0; v < L::kNv; ++v)
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const int c = L::at(v, t) + i;
-            w[v * E + i] = a.weight && c < width ? load_param(a.weight, a.w_type, c) : 1.f;
-            b[v * E + i] = a.bias && c < width ? load_param(a.bias, a.w_type, c) : 0.f;
-        }
     const long long step = static_cast<long long>(gridDim.x) * L::kRows;
     long long base = static_cast<long long>(blockIdx.x) * L::kRows;
     auto fetch = [&](long long row, int slot) {   // one group of copies, empty behind the last row
@@ -227,6 +239,12 @@ k_norm_fwd(FwdArgs a) {
     };
 #pragma unroll
     for (int q = 0; q < S; ++q) fetch(base + threadIdx.x / TPR + q * step, q);
+    float w[EPT], b[EPT];   // behind the first rows' copies, which take as long
+#pragma unroll
+    for (int v = 0; v < L::kNv; ++v) {
+        load_params<E>(w + v * E, a.weight, a.w_type, L::at(v, t), width, a.w_wide, 1.f);
+        load_params<E>(b + v * E, a.bias, a.w_type, L::at(v, t), width, a.w_wide, 0.f);
+    }
     for (int slot = 0; base < a.rows; base += step) {   // the same number of turns for all threads of a block
         const long long row = base + threadIdx.x / TPR;
         const bool live = row < a.rows;
@@ -307,15 +325,6 @@ k_norm_bwd(BwdArgs a) {
     int half = 0;
     const int t = threadIdx.x % TPR, width = static_cast<int>(a.width);
     const float inv = 1.f / static_cast<float>(width);
-    float w[EPT], dw[EPT], db[EPT];
-#pragma unroll
-    for (int v = 0; v < L::kNv; ++v)
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const int c = L::at(v, t) + i;
-            w[v * E + i] = a.weight && c < width ? load_param(a.weight, a.w_type, c) : 1.f;
-            dw[v * E + i] = db[v * E + i] = 0.f;
-        }
     const long long step = static_cast<long long>(gridDim.x) * L::kRows;
     long long base = static_cast<long long>(blockIdx.x) * L::kRows;
     auto fetch = [&](long long row, int slot) {
@@ -338,6 +347,11 @@ k_norm_bwd(BwdArgs a) {
     };
 #pragma unroll
     for (int q = 0; q < S; ++q) fetch(base + threadIdx.x / TPR + q * step, q);
+    float w[EPT], dw[EPT], db[EPT];
+#pragma unroll
+    for (int v = 0; v < L::kNv; ++v) load_params<E>(w + v * E, a.weight, a.w_type, L::at(v, t), width, a.w_wide, 1.f);
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) dw[e] = db[e] = 0.f;
     float2 st = make_float2(0.f, 0.f);
     if (base + threadIdx.x / TPR < a.rows) st = a.stats[base + threadIdx.x / TPR];
     for (int slot = 0; base < a.rows; base += step) {
@@ -405,26 +419,25 @@ k_norm_bwd(BwdArgs a) {
     }
     if (!a.part) return;
     // the block's rows side by side: their column sums, in the order of the groups
-    float* cols = reinterpret_cast<float*>(ring);   // [2][TPR * EPT]; no copy is under way any more
+    float* cols = reinterpret_cast<float*>(ring);   // [rows of the block][2][TPR * EPT]; no copy is under way any more
     if constexpr (VEC) copies_wait<0>();
     __syncthreads();
-    for (int q = 0; q < L::kRows; ++q) {
-        if (static_cast<int>(threadIdx.x) / TPR == q) {
+    float* mine = cols + threadIdx.x / TPR * 2 * TPR * EPT;
 #pragma unroll
-            for (int v = 0; v < L::kNv; ++v)
+    for (int v = 0; v < L::kNv; ++v)
 #pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    const int c = L::at(v, t) + i, e = v * E + i;
-                    cols[c] = q ? cols[c] + dw[e] : dw[e];
-                    cols[TPR * EPT + c] = q ? cols[TPR * EPT + c] + db[e] : db[e];
-                }
+        for (int i = 0; i < E; ++i) {
+            mine[L::at(v, t) + i] = dw[v * E + i];
+            mine[TPR * EPT + L::at(v, t) + i] = db[v * E + i];
         }
-        __syncthreads();
-    }
+    __syncthreads();
     float* part = a.part + static_cast<long long>(blockIdx.x) * 2 * width;
-    for (int c = threadIdx.x; c < width; c += B) {
-        part[c] = cols[c];
-        part[width + c] = cols[TPR * EPT + c];
+    for (int c = threadIdx.x; c < 2 * width; c += B) {
+        const int at = c < width ? c : c - width + TPR * EPT;
+        float sum = cols[at];
+#pragma unroll
+        for (int q = 1; q < L::kRows; ++q) sum += cols[q * 2 * TPR * EPT + at];
+        part[c] = sum;
     }
 }
 
@@ -517,21 +530,24 @@ __global__ void __launch_bounds__(kThreads) k_norm_dw_wide(BwdArgs a) {
     }
 }
 
-// The partial sums of 32 columns per block, 8 runs of them side by side and then in order: the result does not depend on
-// which block ran when.
-__global__ void __launch_bounds__(kThreads) k_norm_dw_sum(BwdArgs a) {
-    __shared__ float red[kThreads / 32][32];
-    const long long i = static_cast<long long>(blockIdx.x) * 32 + (threadIdx.x & 31);
-    const int q = threadIdx.x >> 5;
+// The partial sums of 32 columns per block, 32 runs of them side by side and then in order: the result does not depend on
+// which block ran when. (8 runs per block took 6.0 us for 296 partial sums of 512 columns, 32 take 3.3 us.)
+__global__ void __launch_bounds__(1024) k_norm_dw_sum(BwdArgs a) {
+    __shared__ float red[32][33];
+    const int c = threadIdx.x & 31, q = threadIdx.x >> 5;
+    const long long i = static_cast<long long>(blockIdx.x) * 32 + c;
     float t = 0.f;
-    if (i < 2 * a.width)
-        for (int p = q; p < a.splits; p += kThreads / 32) t += a.part[static_cast<long long>(p) * 2 * a.width + i];
-    red[q][threadIdx.x & 31] = t;
+    if (i < 2 * a.width) {
+#pragma unroll 4
+        for (int p = q; p < a.splits; p += 32) t += a.part[static_cast<long long>(p) * 2 * a.width + i];
+    }
+    red[q][c] = t;
     __syncthreads();
-    if (q == 0 && i < 2 * a.width) {
-        for (int j = 1; j < kThreads / 32; ++j) t += red[j][threadIdx.x];
-        void* out = i < a.width ? a.dweight : a.dbias;
-        if (out) store_param(out, a.w_type, i < a.width ? i : i - a.width, t);
+    t = warp_sum(red[c][q]);   // column q of the block
+    const long long col = static_cast<long long>(blockIdx.x) * 32 + q;
+    if (c == 0 && col < 2 * a.width) {
+        void* out = col < a.width ? a.dweight : a.dbias;
+        if (out) store_param(out, a.w_type, col < a.width ? col : col - a.width, t);
     }
 }
 
@@ -647,7 +663,7 @@ int rl_norm_fwd(const void* x, const void* residual, const void* weight, const v
     if (const char* e = bad_shape(rows, width, x_type, y_type, w_type)) return failed(e);
     if (rows == 0) return 0;
     if (!x || !y || (residual && !sum)) return failed("x, y and (with a residual) sum must be given");
-    FwdArgs a{x, residual, weight, bias, y, sum, static_cast<float2*>(stats), rows, width, x_stride, r_stride, w_type, eps};
+    FwdArgs a{x, residual, weight, bias, y, sum, static_cast<float2*>(stats), rows, width, x_stride, r_stride, w_type, aligned(weight, 0, w_type) && aligned(bias, 0, w_type), eps};
     auto s = static_cast<cudaStream_t>(stream);
     cudaError_t e = cudaSuccess;
     with_types(x_type, y_type, [&](auto tx, auto ty) {
@@ -687,7 +703,7 @@ int rl_norm_bwd(const void* gy, const void* gsum, const void* s, const void* sta
         return failed("work space smaller than rl_norm_bwd_work_bytes()");
     BwdArgs a{gy, gsum, s, weight, static_cast<const float2*>(stats), dx, dweight, dbias,
               params ? static_cast<float*>(work) : nullptr, rows, width, gy_stride, gsum_stride, s_stride, w_type,
-              splits_of(rows, width)};
+              aligned(weight, 0, w_type), splits_of(rows, width)};
     if (!dx && !params) return 0;
     auto q = static_cast<cudaStream_t>(stream);
     cudaError_t e = cudaSuccess;
@@ -712,7 +728,7 @@ int rl_norm_bwd(const void* gy, const void* gsum, const void* s, const void* sta
                     : launch<k_norm_bwd<TX, TY, false, tpr(), ept()>>(grid, N::kBlock, N::kSmem, q, a);
         });
     });
-    if (e == cudaSuccess && params) k_norm_dw_sum<<<static_cast<unsigned>((2 * width + 31) / 32), kThreads, 0, q>>>(a);
+    if (e == cudaSuccess && params) k_norm_dw_sum<<<static_cast<unsigned>((2 * width + 31) / 32), 1024, 0, q>>>(a);
     if (e == cudaSuccess) e = cudaGetLastError();
     return e == cudaSuccess ? 0 : failed(cudaGetErrorString(e));
 }

@@ -18,6 +18,7 @@
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kWideThreads = 512;
 constexpr int kDevices = 64;                               // whose properties are kept
 constexpr int kMaxRow = 8192;                              // values of a row that a block's registers hold
 constexpr int kCols = 64, kColRows = kThreads / kCols;
@@ -117,20 +118,41 @@ template <class T, int N>
 __device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
     return *reinterpret_cast<const Pack<T, N>*>(p);
 }
+// Values rounded to T, two at a time where T has an instruction for two.
+template <class T, int N>
+__device__ __forceinline__ Pack<T, N> rounded(const float* v) {
+    Pack<T, N> q;
+    if constexpr (N % 2 == 0 && sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            if constexpr (std::is_same_v<T, __nv_bfloat16>) *reinterpret_cast<__nv_bfloat162*>(q.v + i) = __floats2bfloat162_rn(v[i], v[i + 1]);
+            else *reinterpret_cast<__half2*>(q.v + i) = __floats2half2_rn(v[i], v[i + 1]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) q.v[i] = from_f<T>(v[i]);
+    }
+    return q;
+}
 template <class T, int N>
 __device__ __forceinline__ void store_pack(T* p, const float* v) {
-    Pack<T, N> q;
-#pragma unroll
-    for (int i = 0; i < N; ++i) q.v[i] = from_f<T>(v[i]);
-    *reinterpret_cast<Pack<T, N>*>(p) = q;
+    *reinterpret_cast<Pack<T, N>*>(p) = rounded<T, N>(v);
 }
 
-// The sums of two values over a row's TPR threads, in each of them. `red` has two places for each warp of the block and is
-// free again at the next but one call: the calls alternate between its two halves.
+// The sum over the TPR <= 32 lanes that share a row, in each of them.
+template <int TPR>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+    for (int o = (TPR < 32 ? TPR : 32) / 2; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    return v;
+}
+
+// The sums of one or two values over a row's TPR threads, in each of them. `red` has a place for each warp of the block, and
+// is free again at the next but one call: the calls alternate between its two halves.
 template <int TPR>
 __device__ __forceinline__ float2 row_sums(float x, float y, float2* red) {
-    x = warp_sum(x);
-    y = warp_sum(y);
+    x = lanes_sum<TPR>(x);
+    y = lanes_sum<TPR>(y);
     if constexpr (TPR > 32) {
         const int warp = threadIdx.x >> 5, first = warp & ~(TPR / 32 - 1);
         if ((threadIdx.x & 31) == 0) red[warp] = make_float2(x, y);
@@ -147,7 +169,7 @@ __device__ __forceinline__ float2 row_sums(float x, float y, float2* red) {
 
 template <int TPR>
 __device__ __forceinline__ float row_sum(float x, float* red) {
-    x = warp_sum(x);
+    x = lanes_sum<TPR>(x);
     if constexpr (TPR > 32) {
         const int warp = threadIdx.x >> 5, first = warp & ~(TPR / 32 - 1);
         if ((threadIdx.x & 31) == 0) red[warp] = x;
@@ -209,97 +231,104 @@ struct Bwd : Tile<TX, VEC, TPR, EPT> {
     static constexpr size_t kSmem = kRing > kCols ? kRing : kCols;
 };
 
+// Rows go to teams of TPR threads; the lanes of a warp (teams within one) and the warps of a block (teams of several) take
+// the same number of turns. A team behind the last row works on that row again, and writes nothing.
 template <class TX, class TY, bool VEC, int TPR, int EPT>
 __global__ void __launch_bounds__(Fwd<TX, TY, VEC, TPR, EPT>::kBlock, kFwdWarps * 32 / Fwd<TX, TY, VEC, TPR, EPT>::kBlock)
 k_norm_fwd(FwdArgs a) {
     using L = Fwd<TX, TY, VEC, TPR, EPT>;
     using P = Pack<TX, L::kVe>;
-    constexpr int B = L::kBlock, S = L::kDepth, W = L::kW, E = L::kVe;
+    constexpr int B = L::kBlock, S = L::kDepth, W = L::kW, E = L::kVe, NV = L::kNv;
     extern __shared__ uint4 ring[];   // [S][x, residual][W][B]
     __shared__ float red[2][B / 32];
     const int t = threadIdx.x % TPR, width = static_cast<int>(a.width);
     const float inv = 1.f / static_cast<float>(width);
     const long long step = static_cast<long long>(gridDim.x) * L::kRows;
-    long long base = static_cast<long long>(blockIdx.x) * L::kRows;
-    auto fetch = [&](long long row, int slot) {   // one group of copies, empty behind the last row
+    long long row = static_cast<long long>(blockIdx.x) * L::kRows + threadIdx.x / TPR;   // this team's
+    long long first = row - (TPR < 32 ? (threadIdx.x & 31) / TPR : TPR == 32 ? 0 : threadIdx.x / TPR);
+    auto fetch = [&](long long at_row, int slot) {   // one group of copies, empty behind the last row
         if constexpr (VEC) {
-            if (row < a.rows) {
-                const TX* px = static_cast<const TX*>(a.x) + row * a.x_stride;
-                const TX* pr = static_cast<const TX*>(a.res) + row * a.r_stride;
+            if (at_row < a.rows) {
+                const TX* px = static_cast<const TX*>(a.x) + at_row * a.x_stride;
+                const TX* pr = static_cast<const TX*>(a.res) + at_row * a.r_stride;
                 uint4* at = ring + slot * 2 * W * B + threadIdx.x;
 #pragma unroll
-                for (int v = 0; v < L::kNv; ++v)
+                for (int v = 0; v < NV; ++v)
                     if (L::at(v, t) < width) {
-                        copy_pack<TX, E, B>(at + v * (W / L::kNv) * B, px + L::at(v, t));
-                        if (a.res) copy_pack<TX, E, B>(at + (W + v * (W / L::kNv)) * B, pr + L::at(v, t));
+                        copy_pack<TX, E, B>(at + v * (W / NV) * B, px + L::at(v, t));
+                        if (a.res) copy_pack<TX, E, B>(at + (W + v * (W / NV)) * B, pr + L::at(v, t));
                     }
             }
             copies_commit();
         }
     };
 #pragma unroll
-    for (int q = 0; q < S; ++q) fetch(base + threadIdx.x / TPR + q * step, q);
+    for (int q = 0; q < S; ++q) fetch(row + q * step, q);
     float w[EPT], b[EPT];   // behind the first rows' copies, which take as long
 #pragma unroll
-    for (int v = 0; v < L::kNv; ++v) {
+    for (int v = 0; v < NV; ++v) {
         load_params<E>(w + v * E, a.weight, a.w_type, L::at(v, t), width, a.w_wide, 1.f);
         load_params<E>(b + v * E, a.bias, a.w_type, L::at(v, t), width, a.w_wide, 0.f);
     }
-    for (int slot = 0; base < a.rows; base += step) {   // the same number of turns for all threads of a block
-        const long long row = base + threadIdx.x / TPR;
+    for (int slot = 0; first < a.rows; first += step, row += step) {
         const bool live = row < a.rows;
-        const TX* px = static_cast<const TX*>(a.x) + row * a.x_stride;
-        const TX* pr = static_cast<const TX*>(a.res) + row * a.r_stride;
-        const uint4* at = ring + slot * 2 * W * B + threadIdx.x;
+        const long long from = live ? row : a.rows - 1;
         if constexpr (VEC) copies_wait<S - 1>();
-        float s[EPT];
-        float sum = 0.f;
+        P x[NV];
 #pragma unroll
-        for (int v = 0; v < L::kNv; ++v) {
-            const bool in = live && L::at(v, t) < width;
-            P x, r;
-            if (in) {
-                if constexpr (VEC) {
-                    x = slot_pack<TX, E, B>(at + v * (W / L::kNv) * B);
-                    if (a.res) r = slot_pack<TX, E, B>(at + (W + v * (W / L::kNv)) * B);
-                } else {
-                    x = load_pack<TX, E>(px + L::at(v, t));
-                    if (a.res) r = load_pack<TX, E>(pr + L::at(v, t));
+        for (int v = 0; v < NV; ++v) {
+            x[v] = P{};
+            if (L::at(v, t) < width) {
+                if constexpr (VEC) x[v] = slot_pack<TX, E, B>(ring + (slot * 2 * W + v * (W / NV)) * B + threadIdx.x);
+                else x[v] = load_pack<TX, E>(static_cast<const TX*>(a.x) + from * a.x_stride + L::at(v, t));
+            }
+        }
+        if (a.res) {
+            P r[NV];
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                r[v] = P{};
+                if (L::at(v, t) < width) {
+                    if constexpr (VEC) r[v] = slot_pack<TX, E, B>(ring + (slot * 2 * W + W + v * (W / NV)) * B + threadIdx.x);
+                    else r[v] = load_pack<TX, E>(static_cast<const TX*>(a.res) + from * a.r_stride + L::at(v, t));
                 }
             }
+            TX* ps = static_cast<TX*>(a.sum) + row * width;
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                float q = in ? to_f(x.v[i]) : 0.f;
-                if (a.res) q = in ? to_f(from_f<TX>(q + to_f(r.v[i]))) : 0.f;
-                s[v * E + i] = q;
-                sum += q;
+            for (int v = 0; v < NV; ++v) {
+                float q[E];
+#pragma unroll
+                for (int i = 0; i < E; ++i) q[i] = to_f(x[v].v[i]) + to_f(r[v].v[i]);
+                x[v] = rounded<TX, E>(q);
+                if (live && L::at(v, t) < width) *reinterpret_cast<P*>(ps + L::at(v, t)) = x[v];
             }
         }
         if constexpr (VEC) {
             fetch(row + S * step, slot);
             slot = slot + 1 == S ? 0 : slot + 1;
         }
-        if (a.res && live) {
-            TX* ps = static_cast<TX*>(a.sum) + row * width;
+        float s[EPT];
+        float sum = 0.f;
 #pragma unroll
-            for (int v = 0; v < L::kNv; ++v)
-                if (L::at(v, t) < width) store_pack<TX, E>(ps + L::at(v, t), s + v * E);
-        }
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int i = 0; i < E; ++i) sum += s[v * E + i] = to_f(x[v].v[i]);
         const float mu = row_sum<TPR>(sum, red[0]) * inv;
         float sq = 0.f;
 #pragma unroll
-        for (int v = 0; v < L::kNv; ++v)
+        for (int v = 0; v < NV; ++v)
+            if (L::at(v, t) < width) {
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                float& q = s[v * E + i];
-                q = L::at(v, t) < width ? q - mu : 0.f;
-                sq = fmaf(q, q, sq);
+                for (int i = 0; i < E; ++i) {
+                    s[v * E + i] -= mu;
+                    sq = fmaf(s[v * E + i], s[v * E + i], sq);
+                }
             }
         const float rs = rsqrtf(fmaf(row_sum<TPR>(sq, red[1]), inv, a.eps));
         if (!live) continue;
         TY* py = static_cast<TY*>(a.y) + row * width;
 #pragma unroll
-        for (int v = 0; v < L::kNv; ++v)
+        for (int v = 0; v < NV; ++v)
             if (L::at(v, t) < width) {
                 float y[E];
 #pragma unroll
@@ -311,103 +340,120 @@ k_norm_fwd(FwdArgs a) {
 }
 
 // Both gradients in one pass over gy and s: each thread also sums its columns' gy xh and gy over the rows that it sees, and
-// the block writes their sums once, a.splits blocks in all. The row's values are taken from shared memory a second time
-// when their means are known, not kept in registers.
+// the block writes their sums once, a.splits blocks in all. The row's values are read a second time, from shared memory (or
+// L1), when their means are known, not kept in registers.
 template <class TX, class TY, bool VEC, int TPR, int EPT>
 __global__ void __launch_bounds__(Bwd<TX, TY, VEC, TPR, EPT>::kBlock, kBwdWarps * 32 / Bwd<TX, TY, VEC, TPR, EPT>::kBlock)
 k_norm_bwd(BwdArgs a) {
     using L = Bwd<TX, TY, VEC, TPR, EPT>;
     using PX = Pack<TX, L::kVe>;
     using PY = Pack<TY, L::kVe>;
-    constexpr int B = L::kBlock, S = L::kDepth, W = L::kW, G = L::kG, E = L::kVe, R = 2 * W + G;
+    constexpr int B = L::kBlock, S = L::kDepth, W = L::kW, G = L::kG, E = L::kVe, NV = L::kNv, R = 2 * W + G;
     extern __shared__ uint4 ring[];   // [S][s, gsum, gy][W, W, G][B]
     __shared__ float2 red[2][B / 32];
     int half = 0;
     const int t = threadIdx.x % TPR, width = static_cast<int>(a.width);
     const float inv = 1.f / static_cast<float>(width);
     const long long step = static_cast<long long>(gridDim.x) * L::kRows;
-    long long base = static_cast<long long>(blockIdx.x) * L::kRows;
-    auto fetch = [&](long long row, int slot) {
+    long long row = static_cast<long long>(blockIdx.x) * L::kRows + threadIdx.x / TPR;
+    long long first = row - (TPR < 32 ? (threadIdx.x & 31) / TPR : TPR == 32 ? 0 : threadIdx.x / TPR);
+    auto fetch = [&](long long at_row, int slot) {
         if constexpr (VEC) {
-            if (row < a.rows) {
-                const TX* ps = static_cast<const TX*>(a.s) + row * a.s_stride;
-                const TX* pq = static_cast<const TX*>(a.gsum) + row * a.gsum_stride;
-                const TY* pg = static_cast<const TY*>(a.gy) + row * a.gy_stride;
+            if (at_row < a.rows) {
+                const TX* ps = static_cast<const TX*>(a.s) + at_row * a.s_stride;
+                const TX* pq = static_cast<const TX*>(a.gsum) + at_row * a.gsum_stride;
+                const TY* pg = static_cast<const TY*>(a.gy) + at_row * a.gy_stride;
                 uint4* at = ring + slot * R * B + threadIdx.x;
 #pragma unroll
-                for (int v = 0; v < L::kNv; ++v)
+                for (int v = 0; v < NV; ++v)
                     if (L::at(v, t) < width) {
-                        copy_pack<TX, E, B>(at + v * (W / L::kNv) * B, ps + L::at(v, t));
-                        if (a.gsum) copy_pack<TX, E, B>(at + (W + v * (W / L::kNv)) * B, pq + L::at(v, t));
-                        copy_pack<TY, E, B>(at + (2 * W + v * (G / L::kNv)) * B, pg + L::at(v, t));
+                        copy_pack<TX, E, B>(at + v * (W / NV) * B, ps + L::at(v, t));
+                        if (a.gsum) copy_pack<TX, E, B>(at + (W + v * (W / NV)) * B, pq + L::at(v, t));
+                        copy_pack<TY, E, B>(at + (2 * W + v * (G / NV)) * B, pg + L::at(v, t));
                     }
             }
             copies_commit();
         }
     };
 #pragma unroll
-    for (int q = 0; q < S; ++q) fetch(base + threadIdx.x / TPR + q * step, q);
+    for (int q = 0; q < S; ++q) fetch(row + q * step, q);
     float w[EPT], dw[EPT], db[EPT];
 #pragma unroll
-    for (int v = 0; v < L::kNv; ++v) load_params<E>(w + v * E, a.weight, a.w_type, L::at(v, t), width, a.w_wide, 1.f);
+    for (int v = 0; v < NV; ++v) load_params<E>(w + v * E, a.weight, a.w_type, L::at(v, t), width, a.w_wide, 1.f);
 #pragma unroll
     for (int e = 0; e < EPT; ++e) dw[e] = db[e] = 0.f;
-    float2 st = make_float2(0.f, 0.f);
-    if (base + threadIdx.x / TPR < a.rows) st = a.stats[base + threadIdx.x / TPR];
-    for (int slot = 0; base < a.rows; base += step) {
-        const long long row = base + threadIdx.x / TPR;
+    float2 st = a.stats[row < a.rows ? row : a.rows - 1];
+    for (int slot = 0; first < a.rows; first += step, row += step) {
         const bool live = row < a.rows;
-        const TX* ps = static_cast<const TX*>(a.s) + row * a.s_stride;
-        const TX* pq = static_cast<const TX*>(a.gsum) + row * a.gsum_stride;
-        const TY* pg = static_cast<const TY*>(a.gy) + row * a.gy_stride;
+        const long long from = live ? row : a.rows - 1;
+        const TX* ps = static_cast<const TX*>(a.s) + from * a.s_stride;
+        const TX* pq = static_cast<const TX*>(a.gsum) + from * a.gsum_stride;
+        const TY* pg = static_cast<const TY*>(a.gy) + from * a.gy_stride;
         const uint4* at = ring + slot * R * B + threadIdx.x;
         auto value_s = [&](int v) -> PX {
-            if constexpr (VEC) return slot_pack<TX, E, B>(at + v * (W / L::kNv) * B);
+            if constexpr (VEC) return slot_pack<TX, E, B>(at + v * (W / NV) * B);
             else return load_pack<TX, E>(ps + L::at(v, t));
         };
         auto value_q = [&](int v) -> PX {
-            if constexpr (VEC) return slot_pack<TX, E, B>(at + (W + v * (W / L::kNv)) * B);
+            if constexpr (VEC) return slot_pack<TX, E, B>(at + (W + v * (W / NV)) * B);
             else return load_pack<TX, E>(pq + L::at(v, t));
         };
         auto value_g = [&](int v) -> PY {
-            if constexpr (VEC) return slot_pack<TY, E, B>(at + (2 * W + v * (G / L::kNv)) * B);
+            if constexpr (VEC) return slot_pack<TY, E, B>(at + (2 * W + v * (G / NV)) * B);
             else return load_pack<TY, E>(pg + L::at(v, t));
         };
         if constexpr (VEC) copies_wait<S - 1>();
         const float mu = st.x, rs = st.y;
         if (row + step < a.rows) st = a.stats[row + step];
         float th = 0.f, thx = 0.f;
+        if (live) {
+            PX s[VEC ? 1 : NV];
+            PY g[VEC ? 1 : NV];
+            if constexpr (!VEC) {   // all loads before their first use
 #pragma unroll
-        for (int v = 0; v < L::kNv; ++v)
-            if (live && L::at(v, t) < width) {
-                const PX s = value_s(v);
-                const PY g = value_g(v);
-#pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    const int e = v * E + i;
-                    const float q = to_f(g.v[i]), xh = (to_f(s.v[i]) - mu) * rs, h = q * w[e];
-                    dw[e] = fmaf(q, xh, dw[e]);
-                    db[e] += q;
-                    th += h;
-                    thx = fmaf(h, xh, thx);
-                }
+                for (int v = 0; v < NV; ++v)
+                    if (L::at(v, t) < width) {
+                        s[v] = value_s(v);
+                        g[v] = value_g(v);
+                    }
             }
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+                if (L::at(v, t) < width) {
+                    if constexpr (VEC) {
+                        s[0] = value_s(v);
+                        g[0] = value_g(v);
+                    }
+#pragma unroll
+                    for (int i = 0; i < E; ++i) {
+                        const int e = v * E + i;
+                        const float q = to_f(g[VEC ? 0 : v].v[i]), xh = (to_f(s[VEC ? 0 : v].v[i]) - mu) * rs, h = q * w[e];
+                        dw[e] = fmaf(q, xh, dw[e]);
+                        db[e] += q;
+                        th += h;
+                        thx = fmaf(h, xh, thx);
+                    }
+                }
+        }
         const float2 sums = row_sums<TPR>(th, thx, red[half ^= 1]);
         const float mh = sums.x * inv, mhx = sums.y * inv;
         if (live && a.dx) {
             TX* pd = static_cast<TX*>(a.dx) + row * width;
 #pragma unroll
-            for (int v = 0; v < L::kNv; ++v)
+            for (int v = 0; v < NV; ++v)
                 if (L::at(v, t) < width) {
                     const PX s = value_s(v);
                     const PY g = value_g(v);
-                    PX q;
-                    if (a.gsum) q = value_q(v);
                     float d[E];
 #pragma unroll
                     for (int i = 0; i < E; ++i) {
                         const float xh = (to_f(s.v[i]) - mu) * rs;
-                        d[i] = fmaf(fmaf(-xh, mhx, to_f(g.v[i]) * w[v * E + i] - mh), rs, a.gsum ? to_f(q.v[i]) : 0.f);
+                        d[i] = fmaf(-xh, mhx, to_f(g.v[i]) * w[v * E + i] - mh) * rs;
+                    }
+                    if (a.gsum) {
+                        const PX q = value_q(v);
+#pragma unroll
+                        for (int i = 0; i < E; ++i) d[i] += to_f(q.v[i]);
                     }
                     store_pack<TX, E>(pd + L::at(v, t), d);
                 }
@@ -442,61 +488,108 @@ k_norm_bwd(BwdArgs a) {
 }
 
 // ------------------------------------------------------------------ wider rows: read again for each pass
+//
+// A block per row, N neighbouring values per thread and turn (16 bytes, or one where the rows are not aligned).
 
-template <class TX, class TY>
-__global__ void __launch_bounds__(kThreads) k_norm_fwd_wide(FwdArgs a) {
-    __shared__ float red[2][kThreads / 32];
+template <class TX, class TY, int N>
+__global__ void __launch_bounds__(kWideThreads) k_norm_fwd_wide(FwdArgs a) {
+    __shared__ float red[2][kWideThreads / 32];
     const float inv = 1.f / static_cast<float>(a.width);
+    const int width = static_cast<int>(a.width), start = threadIdx.x * N;
+    constexpr int kStep = kWideThreads * N;
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const TX* x = static_cast<const TX*>(a.x) + row * a.x_stride;
         if (a.res) {
             const TX* r = static_cast<const TX*>(a.res) + row * a.r_stride;
             TX* s = static_cast<TX*>(a.sum) + row * a.width;
-            for (long long i = threadIdx.x; i < a.width; i += kThreads) s[i] = from_f<TX>(to_f(x[i]) + to_f(r[i]));
+#pragma unroll 4
+            for (int i = start; i < width; i += kStep) {
+                const Pack<TX, N> p = load_pack<TX, N>(x + i), q = load_pack<TX, N>(r + i);
+                float v[N];
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[e] = to_f(p.v[e]) + to_f(q.v[e]);
+                store_pack<TX, N>(s + i, v);
+            }
             x = s;   // each thread reads back only what it wrote itself
         }
         float t = 0.f;
-        for (long long i = threadIdx.x; i < a.width; i += kThreads) t += to_f(x[i]);
-        const float mu = row_sum<kThreads>(t, red[0]) * inv;
-        t = 0.f;
-        for (long long i = threadIdx.x; i < a.width; i += kThreads) {
-            const float c = to_f(x[i]) - mu;
-            t = fmaf(c, c, t);
+#pragma unroll 4
+        for (int i = start; i < width; i += kStep) {
+            const Pack<TX, N> p = load_pack<TX, N>(x + i);
+#pragma unroll
+            for (int e = 0; e < N; ++e) t += to_f(p.v[e]);
         }
-        const float rs = rsqrtf(fmaf(row_sum<kThreads>(t, red[1]), inv, a.eps));
+        const float mu = row_sum<kWideThreads>(t, red[0]) * inv;
+        t = 0.f;
+#pragma unroll 4
+        for (int i = start; i < width; i += kStep) {
+            const Pack<TX, N> p = load_pack<TX, N>(x + i);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float c = to_f(p.v[e]) - mu;
+                t = fmaf(c, c, t);
+            }
+        }
+        const float rs = rsqrtf(fmaf(row_sum<kWideThreads>(t, red[1]), inv, a.eps));
         TY* y = static_cast<TY*>(a.y) + row * a.width;
-        for (long long i = threadIdx.x; i < a.width; i += kThreads) {
-            const float w = a.weight ? load_param(a.weight, a.w_type, i) : 1.f;
-            const float b = a.bias ? load_param(a.bias, a.w_type, i) : 0.f;
-            y[i] = from_f<TY>(fmaf((to_f(x[i]) - mu) * rs, w, b));
+#pragma unroll 2
+        for (int i = start; i < width; i += kStep) {
+            const Pack<TX, N> p = load_pack<TX, N>(x + i);
+            float w[N], b[N], v[N];
+            load_params<N>(w, a.weight, a.w_type, i, width, a.w_wide, 1.f);
+            load_params<N>(b, a.bias, a.w_type, i, width, a.w_wide, 0.f);
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = fmaf((to_f(p.v[e]) - mu) * rs, w[e], b[e]);
+            store_pack<TY, N>(y + i, v);
         }
         if (a.stats && threadIdx.x == 0) a.stats[row] = make_float2(mu, rs);
     }
 }
 
-template <class TX, class TY>
-__global__ void __launch_bounds__(kThreads) k_norm_dx_wide(BwdArgs a) {
-    __shared__ float2 red[2][kThreads / 32];
+template <class TX, class TY, int N>
+__global__ void __launch_bounds__(kWideThreads) k_norm_dx_wide(BwdArgs a) {
+    __shared__ float2 red[2][kWideThreads / 32];
     int half = 0;
     const float inv = 1.f / static_cast<float>(a.width);
+    const int width = static_cast<int>(a.width), start = threadIdx.x * N;
+    constexpr int kStep = kWideThreads * N;
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const TX* s = static_cast<const TX*>(a.s) + row * a.s_stride;
         const TY* g = static_cast<const TY*>(a.gy) + row * a.gy_stride;
         const float2 st = a.stats[row];
         float th = 0.f, thx = 0.f;
-        for (long long i = threadIdx.x; i < a.width; i += kThreads) {
-            const float h = to_f(g[i]) * (a.weight ? load_param(a.weight, a.w_type, i) : 1.f);
-            th += h;
-            thx = fmaf(h, (to_f(s[i]) - st.x) * st.y, thx);
+#pragma unroll 2
+        for (int i = start; i < width; i += kStep) {
+            const Pack<TX, N> p = load_pack<TX, N>(s + i);
+            const Pack<TY, N> q = load_pack<TY, N>(g + i);
+            float w[N];
+            load_params<N>(w, a.weight, a.w_type, i, width, a.w_wide, 1.f);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float h = to_f(q.v[e]) * w[e];
+                th += h;
+                thx = fmaf(h, (to_f(p.v[e]) - st.x) * st.y, thx);
+            }
         }
-        const float2 sums = row_sums<kThreads>(th, thx, red[half ^= 1]);
+        const float2 sums = row_sums<kWideThreads>(th, thx, red[half ^= 1]);
         const float mh = sums.x * inv, mhx = sums.y * inv;
         TX* dx = static_cast<TX*>(a.dx) + row * a.width;
         const TX* gs = a.gsum ? static_cast<const TX*>(a.gsum) + row * a.gsum_stride : nullptr;
-        for (long long i = threadIdx.x; i < a.width; i += kThreads) {
-            const float h = to_f(g[i]) * (a.weight ? load_param(a.weight, a.w_type, i) : 1.f);
-            const float xh = (to_f(s[i]) - st.x) * st.y;
-            dx[i] = from_f<TX>(fmaf(fmaf(-xh, mhx, h - mh), st.y, gs ? to_f(gs[i]) : 0.f));
+#pragma unroll 2
+        for (int i = start; i < width; i += kStep) {
+            const Pack<TX, N> p = load_pack<TX, N>(s + i);
+            const Pack<TY, N> q = load_pack<TY, N>(g + i);
+            float w[N], d[N];
+            load_params<N>(w, a.weight, a.w_type, i, width, a.w_wide, 1.f);
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                d[e] = fmaf(-(to_f(p.v[e]) - st.x) * st.y, mhx, to_f(q.v[e]) * w[e] - mh) * st.y;
+            if (gs) {
+                const Pack<TX, N> u = load_pack<TX, N>(gs + i);
+#pragma unroll
+                for (int e = 0; e < N; ++e) d[e] += to_f(u.v[e]);
+            }
+            store_pack<TX, N>(dx + i, d);
         }
     }
 }
@@ -569,7 +662,7 @@ int sm_count() {
 }
 
 // Rows that a block takes at a time.
-int block_rows(long long width) { return width <= 512 ? 8 : width <= 1024 ? 4 : width <= 2048 ? 2 : 1; }
+int block_rows(long long width) { return width <= 64 ? 32 : width <= 128 ? 16 : width <= 512 ? 8 : width <= 1024 ? 4 : width <= 2048 ? 2 : 1; }
 int block_warps(long long width) { return width <= 4096 ? 8 : 16; }
 
 // Partial sums of the parameters' gradients: blocks of k_norm_bwd, or row splits of k_norm_dw_wide.
@@ -617,7 +710,9 @@ int failed(const char* msg) {
 template <class F>
 void with_tile(long long width, F f) {
     using std::integral_constant;
-    if (width <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+    if (width <= 64) f(integral_constant<int, 8>{}, integral_constant<int, 8>{});
+    else if (width <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+    else if (width <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
     else if (width <= 512) f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
     else if (width <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
     else if (width <= 2048) f(integral_constant<int, 128>{}, integral_constant<int, 16>{});
@@ -645,7 +740,7 @@ bool with_types(int x_type, int y_type, F f) {
 
 const char* bad_shape(long long rows, long long width, int x_type, int y_type, int w_type) {
     if (rows < 0) return "rows must not be negative";
-    if (width < 1 || width >= (1ll << 31)) return "width must be 1 .. 2^31 - 1";
+    if (width < 1 || width > (1ll << 30)) return "width must be 1 .. 2^30";
     if (x_type < 0 || x_type > 2 || w_type < 0 || w_type > 2) return "unknown type";
     if (y_type != x_type && y_type != 0) return "y must have x's type or be fp32";
     return nullptr;
@@ -669,12 +764,14 @@ int rl_norm_fwd(const void* x, const void* residual, const void* weight, const v
     with_types(x_type, y_type, [&](auto tx, auto ty) {
         using TX = decltype(tx);
         using TY = decltype(ty);
-        if (width > kMaxRow) {
-            k_norm_fwd_wide<TX, TY><<<blocks_of(rows, 8), kThreads, 0, s>>>(a);
-            return;
-        }
         const bool vec = width * sizeof(TX) % 16 == 0 && aligned(x, x_stride, x_type) && aligned(residual, r_stride, x_type) &&
                          aligned(y, 0, y_type) && aligned(sum, 0, x_type);
+        if (width > kMaxRow) {
+            constexpr int kN = 16 / static_cast<int>(sizeof(TX));
+            if (vec) k_norm_fwd_wide<TX, TY, kN><<<blocks_of(rows, 4), kWideThreads, 0, s>>>(a);
+            else k_norm_fwd_wide<TX, TY, 1><<<blocks_of(rows, 4), kWideThreads, 0, s>>>(a);
+            return;
+        }
         const unsigned grid = blocks_of((rows + block_rows(width) - 1) / block_rows(width), kFwdWarps / block_warps(width));
         with_tile(width, [&](auto tpr, auto ept) {
             using V = Fwd<TX, TY, true, tpr(), ept()>;
@@ -710,16 +807,18 @@ int rl_norm_bwd(const void* gy, const void* gsum, const void* s, const void* sta
     with_types(x_type, y_type, [&](auto tx, auto ty) {
         using TX = decltype(tx);
         using TY = decltype(ty);
+        const bool vec = width * sizeof(TX) % 16 == 0 && aligned(s, s_stride, x_type) && aligned(gy, gy_stride, y_type) &&
+                         aligned(gsum, gsum_stride, x_type) && aligned(dx, 0, x_type);
         if (width > kMaxRow) {
-            if (dx) k_norm_dx_wide<TX, TY><<<blocks_of(rows, 8), kThreads, 0, q>>>(a);
+            constexpr int kN = 16 / static_cast<int>(sizeof(TX));
+            if (dx && vec) k_norm_dx_wide<TX, TY, kN><<<blocks_of(rows, 4), kWideThreads, 0, q>>>(a);
+            else if (dx) k_norm_dx_wide<TX, TY, 1><<<blocks_of(rows, 4), kWideThreads, 0, q>>>(a);
             if (params) {
                 const dim3 grid(static_cast<unsigned>((width + kCols - 1) / kCols), static_cast<unsigned>(a.splits));
                 k_norm_dw_wide<TX, TY><<<grid, kThreads, 0, q>>>(a);
             }
             return;
         }
-        const bool vec = width * sizeof(TX) % 16 == 0 && aligned(s, s_stride, x_type) && aligned(gy, gy_stride, y_type) &&
-                         aligned(gsum, gsum_stride, x_type) && aligned(dx, 0, x_type);
         with_tile(width, [&](auto tpr, auto ept) {
             using V = Bwd<TX, TY, true, tpr(), ept()>;
             using N = Bwd<TX, TY, false, tpr(), ept()>;

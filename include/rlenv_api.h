@@ -156,7 +156,7 @@ int rl_stem_bwd(const void* grad, const void* obs, const void* emph, const void*
 // a row's own values are adjacent. All pointers are device pointers unless said otherwise; asynchronous on `stream`;
 // non-zero on a bad argument or launch error (message: rl_norm_error / rl_heads_error, thread-local).
 
-// Layer norm over rows of `width` values: s = x, or x + residual rounded to x's type and written to sum [rows, width];
+// Layer norm over rows of `width` (1 .. 2^30) values: s = x, or x + residual rounded to x's type and written to sum [rows, width];
 // y [rows, width] = (s - mean) / sqrt(variance + eps) * weight + bias, of x's type or fp32. weight, bias [width] of
 // w_type, each may be NULL (1 and 0). stats: NULL, or fp32 [rows, 2] = mean and 1 / sqrt(variance + eps) of each row
 // for the backward. fp32 arithmetic, every output rounded once.

@@ -369,60 +369,71 @@ __device__ __forceinline__ float value_of(unsigned k) { return __uint_as_float(k
 
 using u64 = unsigned long long;
 
-// The sum of v over a warp, 16 bits at a time.
-__device__ __forceinline__ u64 warp_total(unsigned v) {
-    return static_cast<u64>(__reduce_add_sync(~0u, v & 0xFFFFu)) + (static_cast<u64>(__reduce_add_sync(~0u, v >> 16)) << 16);
+// The sum of v < 2^43 over a warp, 16 bits at a time.
+__device__ __forceinline__ u64 warp_total(u64 v) {
+    return static_cast<u64>(__reduce_add_sync(~0u, static_cast<unsigned>(v) & 0xFFFFu)) +
+           (static_cast<u64>(__reduce_add_sync(~0u, static_cast<unsigned>(v >> 16))) << 16);
 }
 
 // Sums and the like over the TPR threads of a row: one warp's by its reduction instructions, more warps' (one row per
-// block) through shared memory, in two places that take turns, so that one barrier per call is enough.
+// block) through shared memory, in two places that take turns, so that one barrier per call is enough (integer atomics on
+// one word per call took longer: 80 us against 74 for 2,049 rows of 4,001 with every truncation).
 template <int TPR>
 struct Team {
     static constexpr int kWarps = TPR / 32;
-    u64* place;   // [2][kWarps][2]
-    int turn = 0;
+    struct Shared {
+        u64 word[2][2][kWarps], warp[2][kWarps];
+    };
+    Shared* s;
+    int turn = 0, side = 0;
 
-    __device__ void exchange(u64& a, u64& b, bool first_is_max) {
+    __device__ explicit Team(Shared* shared) : s(shared) {}
+    // a: added up, or (MAX) the largest; b (if PAIR): added up. One warp's values already.
+    template <bool MAX, bool PAIR>
+    __device__ void join(u64& a, u64& b) {
         if constexpr (kWarps > 1) {
-            u64* p = place + turn * kWarps * 2;
+            auto& w = s->word[turn];
             turn ^= 1;
             if ((threadIdx.x & 31) == 0) {
-                p[2 * (threadIdx.x >> 5)] = a;
-                p[2 * (threadIdx.x >> 5) + 1] = b;
+                w[0][threadIdx.x >> 5] = a;
+                if (PAIR) w[1][threadIdx.x >> 5] = b;
             }
             __syncthreads();
-            a = p[0];
-            b = p[1];
+            a = w[0][0];
+            if (PAIR) b = w[1][0];
 #pragma unroll
-            for (int w = 1; w < kWarps; ++w) {
-                a = first_is_max ? (p[2 * w] > a ? p[2 * w] : a) : a + p[2 * w];
-                b += p[2 * w + 1];
+            for (int q = 1; q < kWarps; ++q) {
+                a = MAX ? (w[0][q] > a ? w[0][q] : a) : a + w[0][q];
+                if (PAIR) b += w[1][q];
             }
         }
     }
-    // The sums of v and of n.
-    __device__ void sums(unsigned v, unsigned n, u64& total, unsigned& count) {
-        u64 a = warp_total(v);
-        u64 b = __reduce_add_sync(~0u, n);
-        exchange(a, b, false);
-        total = a;
-        count = static_cast<unsigned>(b);
+    // The sums of v and of n, as one word: 2^12 weights of 2^27, and a count of 2^12.
+    __device__ void sums(u64 v, unsigned n, u64& total, unsigned& count) {
+        u64 a = warp_total(v) | static_cast<u64>(__reduce_add_sync(~0u, n)) << 44, b = 0;
+        join<false, false>(a, b);
+        total = a & ((1ull << 44) - 1);
+        count = static_cast<unsigned>(a >> 44);
     }
-    __device__ u64 sum(unsigned v) {
-        u64 a = warp_total(v);
-        u64 b = 0;
-        exchange(a, b, false);
+    __device__ u64 sum(u64 v) {
+        u64 a = warp_total(v), b = 0;
+        join<false, false>(a, b);
         return a;
     }
     __device__ unsigned count(unsigned n) {
         u64 a = __reduce_add_sync(~0u, n), b = 0;
-        exchange(a, b, false);
+        join<false, false>(a, b);
+        return static_cast<unsigned>(a);
+    }
+    __device__ unsigned largest(unsigned v) {
+        u64 a = __reduce_max_sync(~0u, v), b = 0;
+        join<true, false>(a, b);
         return static_cast<unsigned>(a);
     }
     // The largest v, and the sum of n.
     __device__ unsigned largest(unsigned v, unsigned n, unsigned& count) {
         u64 a = __reduce_max_sync(~0u, v), b = __reduce_add_sync(~0u, n);
-        exchange(a, b, true);
+        join<true, true>(a, b);
         count = static_cast<unsigned>(b);
         return static_cast<unsigned>(a);
     }
@@ -436,8 +447,8 @@ struct Team {
             if ((threadIdx.x & 31) >= o) run += up;
         }
         if constexpr (kWarps > 1) {
-            u64* p = place + turn * kWarps * 2;
-            turn ^= 1;
+            u64* p = s->warp[side];
+            side ^= 1;
             if ((threadIdx.x & 31) == 31) p[threadIdx.x >> 5] = run;
             __syncthreads();
 #pragma unroll
@@ -475,16 +486,16 @@ __device__ __forceinline__ void cut_row(RowTile<TPR, EPT>& r, Team<TPR>& team, u
             if (hi - lo <= 1) break;
             at = value_of(lo + (hi - lo) / 2);
         }
-        unsigned v = 0, c = 0;
+        unsigned v[2] = {0, 0}, c = 0;   // 16 weights of 2^27 each
 #pragma unroll
         for (int e = 0; e < EPT; ++e)
             if (r.l[e] > at) {
-                if (WEIGHTS) v += r.wgt[e];
+                if (WEIGHTS) v[e / 16] += r.wgt[e];
                 ++c;
             }
         u64 total;
         if (WEIGHTS) {
-            team.sums(v, c, total, c);
+            team.sums(EPT > 16 ? static_cast<u64>(v[0]) + v[1] : v[0], c, total, c);
         } else {
             c = team.count(c);
             total = c;
@@ -541,11 +552,11 @@ __device__ __forceinline__ void cut_row(RowTile<TPR, EPT>& r, Team<TPR>& team, u
     if (group > 1) {
         u64 each = 1;
         if (WEIGHTS) {
-            unsigned w = 0, unused;
+            unsigned w = 0;
 #pragma unroll
             for (int e = 0; e < EPT; ++e)
                 if (r.l[e] > low && r.l[e] <= high) w = r.wgt[e];
-            each = team.largest(w, 0, unused);
+            each = team.largest(w);
         }
         const u64 left = reach - above, want = each == 0 ? group : (left + each - 1) / each;
         if (want < group) {   // the first of the group by index
@@ -587,15 +598,14 @@ __device__ __forceinline__ float kth_bound(const RowTile<TPR, EPT>& r, Team<TPR>
         if (n >= each) t |= bit;
         if (n == each) break;
     }
-    unsigned unused;
-    t = ~team.largest(~t, 0, unused);
+    t = ~team.largest(~t);
     const unsigned floor = key_of(-INFINITY);
     return t > floor + 1 ? value_of(t - 1) : -INFINITY;
 }
 
 // Warps per SM that the registers of EPT choices per thread leave room for.
 template <int EPT>
-constexpr int kRowWarps = EPT <= 4 ? 48 : EPT <= 12 ? 32 : 24;
+constexpr int kRowWarps = EPT <= 4 ? 48 : EPT <= 12 ? 32 : EPT <= 16 ? 24 : 16;
 
 // A warp, or a block of TPR threads, per row; the row's values and weights stay in registers. VEC: rows whose four
 // neighbours can be loaded at once.
@@ -603,9 +613,8 @@ template <class T, int TPR, int EPT, bool VEC>
 __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, TPR == 32 ? kRowWarps<EPT> / 8 : kRowWarps<EPT> * 32 / TPR)
 k_rows_sample(RowArgs a) {
     constexpr int kTeams = TPR == 32 ? 8 : 1;
-    __shared__ u64 place[4 * Team<TPR>::kWarps];
-    Team<TPR> team;
-    team.place = place;
+    __shared__ typename Team<TPR>::Shared team_s;
+    Team<TPR> team(&team_s);
     __shared__ uint4 few_s[kTeams][16];
     uint4* few = few_s[TPR == 32 ? threadIdx.x >> 5 : 0];
     const int n = a.width, lane = threadIdx.x & 31;
@@ -629,9 +638,9 @@ k_rows_sample(RowArgs a) {
         if (parts) bits = __ballot_sync(~0u, lane < kBytes && legal[min(lane, kBytes - 1)] != 0);
         RowTile<TPR, EPT> r;
         float m = 0.f;
-        bool careful = false;   // a second turn: the largest legal value is not finite, or a legal one is a NaN
-        unsigned nans = 0;
-        while (true) {
+        // Loads the row and returns this thread's largest value, a NaN if there is one. CAREFUL: where the row's largest legal
+        // value m (NaNs aside) is not finite, what equals it becomes 0 and the rest -inf; NaNs become -inf.
+        auto load = [&](auto careful) {
             float best = -INFINITY;
 #pragma unroll
             for (int s = 0; s < EPT / 4; ++s) {
@@ -672,7 +681,7 @@ k_rows_sample(RowArgs a) {
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
                     float v = ok[p] ? l[p] : -INFINITY;
-                    if (careful) {   // m: the largest that is no NaN; what equals it becomes 0 if it is not finite
+                    if constexpr (decltype(careful)::value) {
                         if (fabsf(m) < INFINITY) v = v == v ? v : -INFINITY;
                         else v = ok[p] && (m < 0.f ? !(v > m) : v == m) ? 0.f : -INFINITY;
                     }
@@ -680,17 +689,20 @@ k_rows_sample(RowArgs a) {
                     best = max_nan(best, v);
                 }
             }
-            const bool bad = best != best;
-            if (bad) {
-                best = -INFINITY;
+            return best;
+        };
+        float best = load(std::false_type{});
+        const bool bad = best != best;
+        if (bad) {
+            best = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < EPT; ++e) best = fmaxf(best, r.l[e]);
-            }
-            unsigned found;
-            m = value_of(team.largest(key_of(best), bad, found));
-            if (careful || (found == 0 && fabsf(m) < INFINITY)) break;
-            nans = found;
-            careful = true;
+            for (int e = 0; e < EPT; ++e) best = fmaxf(best, r.l[e]);
+        }
+        unsigned nans;
+        m = value_of(team.largest(key_of(best), bad, nans));
+        if (nans || !(fabsf(m) < INFINITY)) {   // rare
+            best = load(std::true_type{});
+            m = value_of(team.largest(key_of(best)));
         }
         if (m == -INFINITY) {   // nothing legal
             if ((threadIdx.x & (TPR - 1)) == 0) {
@@ -711,14 +723,14 @@ k_rows_sample(RowArgs a) {
         }
         if (q.top_p < 1.f) {
             const float floor = m - 20.f / q.scale;   // exp(-20) 2^27 rounds to nothing
-            unsigned w = 0, count = 0;
+            unsigned w[2] = {0, 0}, count = 0;
 #pragma unroll
             for (int e = 0; e < EPT; ++e) {
-                w += r.wgt[e];
+                w[e / 16] += r.wgt[e];
                 count += r.l[e] > floor;
             }
             u64 total;
-            team.sums(w, count, total, count);
+            team.sums(EPT > 16 ? static_cast<u64>(w[0]) + w[1] : w[0], count, total, count);
             const double p = ceil(static_cast<double>(q.top_p) * static_cast<double>(total));
             const u64 reach = p < 1.0 ? 1ull : static_cast<u64>(p);
             // choices that could all go together lie below the lowest value that stays: look there first
@@ -1095,9 +1107,9 @@ void with_row_tile(int width, F f) {
     else if (width <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
     else if (width <= 384) f(integral_constant<int, 32>{}, integral_constant<int, 12>{});
     else if (width <= 512) f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
-    else if (width <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
-    else if (width <= 2048) f(integral_constant<int, 128>{}, integral_constant<int, 16>{});
-    else f(integral_constant<int, 256>{}, integral_constant<int, 16>{});
+    else if (width <= 1024) f(integral_constant<int, 32>{}, integral_constant<int, 32>{});
+    else if (width <= 2048) f(integral_constant<int, 64>{}, integral_constant<int, 32>{});
+    else f(integral_constant<int, 128>{}, integral_constant<int, 32>{});
 }
 
 const char* bad_cut(float temperature, const void* temperatures, float top_p, const void* top_ps, float min_p,

@@ -34,6 +34,7 @@ constexpr int kParts = 5, kBytes = 19, kMoves = 324, kTables = 10, kCond = 127;
 constexpr float kScale = 134217728.f;   // 2^27
 constexpr float kUnit = 1.f / kScale;
 constexpr int kThreads = 128;           // and rows of a block's batch
+constexpr int kGradRows = 2;            // rows of a thread at a time in the backward
 constexpr int kDevices = 64;            // whose properties are kept
 constexpr int kMaxWidth = 4096;         // 2^12 weights of 2^27 and a u of 2^24 fit 63 bits
 
@@ -801,16 +802,16 @@ struct LogpArgs {
     long long rows;
 };
 
-template <class T>
+template <class T, int ROWS>
 struct LogpBatch {
-    T logits[kThreads * kBytes];
-    alignas(16) uint8_t masks[kThreads * kBytes];
+    T logits[ROWS * kBytes];
+    alignas(16) uint8_t masks[ROWS * kBytes];
 };
 
-template <class T>
-__device__ __forceinline__ void fetch_batch(const LogpArgs& a, long long first, LogpBatch<T>& to) {
+template <class T, int ROWS>
+__device__ __forceinline__ void fetch_batch(const LogpArgs& a, long long first, LogpBatch<T, ROWS>& to) {
     if (first < a.rows) {
-        const int n = static_cast<int>(min(static_cast<long long>(kThreads), a.rows - first));
+        const int n = static_cast<int>(min(static_cast<long long>(ROWS), a.rows - first));
         stage<kBytes>(to.logits, a.logits, first, n, a.stride, a.dense_logits);
         stage<kBytes>(to.masks, a.masks, first, n, a.mask_stride, a.dense_masks);
     }
@@ -827,58 +828,63 @@ struct SoftRow {
     unsigned some;            // bit k: part k has a legal choice
 };
 
-template <class T>
-__device__ __forceinline__ void soft_row(SoftRow& s, const T* logits, const uint8_t* mask, const float* tab, const int* c) {
-#pragma unroll
-    for (int k = 0; k < kParts; ++k)
-#pragma unroll
-        for (int i = 0; i < part_n(k); ++i) {
-            const int e = part_at(k) + i;
-            float l = to_f(logits[e]);
-            if (tab) {
-#pragma unroll
-                for (int j = 0; j < k; ++j) l += tab[table_at(table_of(k, j)) + c[j] * part_n(k) + i];
-            }
-            s.d[e] = mask[e] != 0 ? l : -INFINITY;
-        }
-    float m[kParts];
+template <int R, class T>
+__device__ __forceinline__ void soft_rows(SoftRow (&s)[R], const T* const (&logits)[R], const uint8_t* const (&mask)[R], const float* tab,
+                                          const int (&c)[R][kParts]) {
+    float m[R][kParts];
     bool odd = false;
 #pragma unroll
-    for (int k = 0; k < kParts; ++k) {
-        m[k] = s.d[part_at(k)];
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int i = 1; i < part_n(k); ++i) m[k] = max_nan(m[k], s.d[part_at(k) + i]);
-        odd |= fabsf(m[k]) == INFINITY;
-    }
-    s.some = 31;
-    if (odd) {
-        float v[kBytes];
+        for (int k = 0; k < kParts; ++k) {
 #pragma unroll
-        for (int e = 0; e < kBytes; ++e) v[e] = s.d[e];
+            for (int i = 0; i < part_n(k); ++i) {
+                const int e = part_at(k) + i;
+                float l = to_f(logits[r][e]);
+                if (tab) {
 #pragma unroll
-        for (int k = 0; k < kParts; ++k)
-            if (fabsf(m[k]) == INFINITY && !settle(v + part_at(k), part_n(k), mask + part_at(k), m[k])) s.some &= ~(1u << k);
-#pragma unroll
-        for (int e = 0; e < kBytes; ++e) s.d[e] = v[e];
-    }
-#pragma unroll
-    for (int k = 0; k < kParts; ++k) {
-        float sum = 0.f, t = 0.f;
-        s.choice_d[k] = 0.f;
-#pragma unroll
-        for (int i = 0; i < part_n(k); ++i) {
-            const int e = part_at(k) + i;
-            const float d = s.d[e] - m[k];
-            if (i == c[k]) s.choice_d[k] = d;
-            s.d[e] = max_nan(d, -200.f);
-            s.w[e] = __expf(s.d[e]);
-            sum += s.w[e];
-            t = fmaf(s.w[e], s.d[e], t);
+                    for (int j = 0; j < k; ++j) l += tab[table_at(table_of(k, j)) + c[r][j] * part_n(k) + i];
+                }
+                s[r].d[e] = mask[r][e] != 0 ? l : -INFINITY;
+                m[r][k] = i == 0 ? s[r].d[e] : max_nan(m[r][k], s[r].d[e]);
+            }
+            odd |= fabsf(m[r][k]) == INFINITY;
         }
-        s.sum[k] = sum;
-        s.inv[k] = __fdividef(1.f, sum);   // the hardware's reciprocal, 1 ulp; S is between 1 and 9
-        s.mean_d[k] = t * s.inv[k];
+#pragma unroll
+    for (int r = 0; r < R; ++r) s[r].some = 31;
+    if (odd) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float v[kBytes];
+#pragma unroll
+            for (int e = 0; e < kBytes; ++e) v[e] = s[r].d[e];
+#pragma unroll
+            for (int k = 0; k < kParts; ++k)
+                if (fabsf(m[r][k]) == INFINITY && !settle(v + part_at(k), part_n(k), mask[r] + part_at(k), m[r][k])) s[r].some &= ~(1u << k);
+#pragma unroll
+            for (int e = 0; e < kBytes; ++e) s[r].d[e] = v[e];
+        }
     }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) {
+            float sum = 0.f, t = 0.f;
+            s[r].choice_d[k] = 0.f;
+#pragma unroll
+            for (int i = 0; i < part_n(k); ++i) {
+                const int e = part_at(k) + i;
+                const float d = s[r].d[e] - m[r][k];
+                if (i == c[r][k]) s[r].choice_d[k] = d;
+                s[r].d[e] = max_nan(d, -200.f);
+                s[r].w[e] = __expf(s[r].d[e]);
+                sum += s[r].w[e];
+                t = fmaf(s[r].w[e], s[r].d[e], t);
+            }
+            s[r].sum[k] = sum;
+            s[r].inv[k] = __fdividef(1.f, sum);   // the hardware's reciprocal, 1 ulp; S is between 1 and 9
+            s[r].mean_d[k] = t * s[r].inv[k];
+        }
 }
 
 __device__ __forceinline__ bool parts_of(int id, int* c) {
@@ -896,7 +902,7 @@ template <class T>
 __global__ void __launch_bounds__(kThreads) k_moves_logp(LogpArgs a) {
     extern __shared__ __align__(16) unsigned char batches[];
     __shared__ float tab_s[kCond];
-    auto* batch = reinterpret_cast<LogpBatch<T>*>(batches);
+    auto* batch = reinterpret_cast<LogpBatch<T, kThreads>*>(batches);
     const long long step = static_cast<long long>(gridDim.x) * kThreads;
     long long first = static_cast<long long>(blockIdx.x) * kThreads;
     fetch_batch(a, first, batch[0]);
@@ -909,12 +915,13 @@ __global__ void __launch_bounds__(kThreads) k_moves_logp(LogpArgs a) {
         copies_wait<1>();
         __syncthreads();
         if (row < a.rows) {
-            int c[kParts];
-            const bool known = parts_of(id, c);   // else no move has this id
-            const T* logits = batch[b].logits + threadIdx.x * kBytes;
-            const uint8_t* mask = batch[b].masks + threadIdx.x * kBytes;
-            SoftRow s;
-            soft_row(s, logits, mask, tab, c);
+            int c[1][kParts];
+            const bool known = parts_of(id, c[0]);   // else no move has this id
+            const T* const logits[1] = {batch[b].logits + threadIdx.x * kBytes};
+            const uint8_t* const mask[1] = {batch[b].masks + threadIdx.x * kBytes};
+            SoftRow rows[1];
+            soft_rows<1>(rows, logits, mask, tab, c);
+            const SoftRow& s = rows[0];
             float d_sum = 0.f, mean_sum = 0.f, sums = 1.f;   // one logarithm for the five parts
 #pragma unroll
             for (int k = 0; k < kParts; ++k)
@@ -931,57 +938,70 @@ __global__ void __launch_bounds__(kThreads) k_moves_logp(LogpArgs a) {
     }
 }
 
-// A thread per row: dl = ga 1[i = c] - p (ga + gb (d - mean_d)), in the logits' place in shared memory and from there to
-// memory as one stretch. Every thread sums the tables' gradient in a column of its own of shared memory (65 KB per block,
-// which leaves 8 warps per SM), so that no two add to one place and the order of the additions is the launch's alone; the
-// 23 additions of a row go to 23 places, so they are read together and written together.
+// dl = ga 1[i = c] - p (ga + gb (d - mean_d)), in the logits' place in shared memory and from there to memory as one stretch.
+// Every thread sums the tables' gradient in a column of its own of shared memory, so that no two add to one place and the
+// order of the additions is the launch's alone; the 23 additions of a row go to 23 places, so they are read together and
+// written together. The columns' 65 KB leave 8 warps per SM, so a thread takes two rows side by side.
 template <class T>
 __global__ void __launch_bounds__(kThreads) k_moves_grad(LogpArgs a) {
-    extern __shared__ __align__(16) unsigned char batches[];   // two batches, then [127][kThreads] sums
+    extern __shared__ __align__(16) unsigned char batches[];   // a batch, then [127][kThreads] sums
     __shared__ float tab_s[kCond];
     __shared__ uint8_t none_s[kBytes];
-    auto* batch = reinterpret_cast<LogpBatch<T>*>(batches);
-    float* acc_s = reinterpret_cast<float*>(batches + 2 * sizeof(LogpBatch<T>));
-    const long long step = static_cast<long long>(gridDim.x) * kThreads;
-    long long first = static_cast<long long>(blockIdx.x) * kThreads;
-    fetch_batch(a, first, batch[0]);
+    constexpr int R = kGradRows, kRows = R * kThreads;
+    auto& batch = *reinterpret_cast<LogpBatch<T, kRows>*>(batches);
+    float* acc_s = reinterpret_cast<float*>(batches + sizeof(batch));
+    const long long step = static_cast<long long>(gridDim.x) * kRows;
+    long long first = static_cast<long long>(blockIdx.x) * kRows;
+    fetch_batch(a, first, batch);
     if (threadIdx.x < kBytes) none_s[threadIdx.x] = 0;
     load_cond(tab_s, a.cond);
     float* acc = a.part ? acc_s + threadIdx.x : nullptr;
     if (acc)
         for (int e = 0; e < kCond; ++e) acc[e * kThreads] = 0.f;
     const float* tab = a.cond.type < 0 ? nullptr : tab_s;
-    for (int b = 0; first < a.rows; first += step, b ^= 1) {
-        fetch_batch(a, first + step, batch[b ^ 1]);
-        const long long row = first + threadIdx.x;
-        float ga = 0.f, gb = 0.f;
-        int id = -1, c[kParts];
-        if (row < a.rows) {
-            id = a.ids[row];
-            if (a.glp) ga = a.glp[row * a.glp_stride];
-            if (a.gent) gb = a.gent[row * a.gent_stride];
+    for (; first < a.rows; first += step) {
+        float ga[R], gb[R];
+        int id[R], c[R][kParts];
+        T* logits[R];
+        const uint8_t* mask[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int at = threadIdx.x + r * kThreads;
+            const long long row = first + at;
+            ga[r] = gb[r] = 0.f;
+            id[r] = -1;
+            if (row < a.rows) {
+                id[r] = a.ids[row];
+                if (a.glp) ga[r] = a.glp[row * a.glp_stride];
+                if (a.gent) gb[r] = a.gent[row * a.gent_stride];
+            }
+            logits[r] = batch.logits + at * kBytes;
+            // behind the last row, or no move's id: nothing is legal, nothing is added
+            mask[r] = parts_of(id[r], c[r]) ? batch.masks + at * kBytes : none_s;
         }
-        copies_wait<1>();
+        copies_wait<0>();
         __syncthreads();
-        T* logits = batch[b].logits + threadIdx.x * kBytes;
-        const uint8_t* mask = batch[b].masks + threadIdx.x * kBytes;
-        if (!parts_of(id, c)) mask = none_s;   // behind the last row, or no move's id: nothing is legal, nothing is added
-        {
-            SoftRow s;
-            soft_row(s, logits, mask, tab, c);
-            float g[kBytes];
+        SoftRow s[R];
+        const T* const from[R] = {logits[0], logits[1]};
+        const uint8_t* const masks[R] = {mask[0], mask[1]};
+        soft_rows<R>(s, from, masks, tab, c);
+        float g[R][kBytes];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int k = 0; k < kParts; ++k) {
-                const bool some = s.some >> k & 1;
-                const int hit = some && mask[part_at(k) + c[k]] != 0 ? c[k] : -1;
-                const float gk = some ? ga : 0.f, bk = some ? gb : 0.f, inv = some ? s.inv[k] : 0.f;
-                const float mean = some ? s.mean_d[k] : 0.f;
+                const bool some = s[r].some >> k & 1;
+                const int hit = some && mask[r][part_at(k) + c[r][k]] != 0 ? c[r][k] : -1;
+                const float gk = some ? ga[r] : 0.f, bk = some ? gb[r] : 0.f, inv = some ? s[r].inv[k] : 0.f;
+                const float mean = some ? s[r].mean_d[k] : 0.f;
 #pragma unroll
                 for (int i = 0; i < part_n(k); ++i) {
                     const int e = part_at(k) + i;
-                    g[e] = fmaf(-s.w[e] * inv, fmaf(bk, s.d[e] - mean, gk), i == hit ? gk : 0.f);
+                    g[r][e] = fmaf(-s[r].w[e] * inv, fmaf(bk, s[r].d[e] - mean, gk), i == hit ? gk : 0.f);
                 }
             }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
             if (acc) {
                 float sum[23];
                 int n = 0;
@@ -991,7 +1011,7 @@ __global__ void __launch_bounds__(kThreads) k_moves_grad(LogpArgs a) {
                     for (int j = 0; j < k; ++j)
 #pragma unroll
                         for (int i = 0; i < part_n(k); ++i)
-                            sum[n++] = acc[(table_at(table_of(k, j)) + c[j] * part_n(k) + i) * kThreads] + g[part_at(k) + i];
+                            sum[n++] = acc[(table_at(table_of(k, j)) + c[r][j] * part_n(k) + i) * kThreads] + g[r][part_at(k) + i];
                 n = 0;
 #pragma unroll
                 for (int k = 1; k < kParts; ++k)
@@ -999,23 +1019,25 @@ __global__ void __launch_bounds__(kThreads) k_moves_grad(LogpArgs a) {
                     for (int j = 0; j < k; ++j)
 #pragma unroll
                         for (int i = 0; i < part_n(k); ++i)
-                            acc[(table_at(table_of(k, j)) + c[j] * part_n(k) + i) * kThreads] = sum[n++];
+                            acc[(table_at(table_of(k, j)) + c[r][j] * part_n(k) + i) * kThreads] = sum[n++];
             }
 #pragma unroll
-            for (int e = 0; e < kBytes; ++e) logits[e] = from_f<T>(g[e]);
+            for (int e = 0; e < kBytes; ++e) logits[r][e] = from_f<T>(g[r][e]);
         }
         __syncthreads();
         if (a.dlogits) {
-            const int n = static_cast<int>(min(static_cast<long long>(kThreads), a.rows - first)) * kBytes;
+            const int n = static_cast<int>(min(static_cast<long long>(kRows), a.rows - first)) * kBytes;
             T* out = static_cast<T*>(a.dlogits) + first * kBytes;
             constexpr int kPer = 16 / static_cast<int>(sizeof(T));
             const int whole = a.dense_out ? n & ~(kPer - 1) : 0;
             for (int i = threadIdx.x * kPer; i < whole; i += kThreads * kPer)
-                *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<const uint4*>(batch[b].logits + i);
-            for (int i = whole + threadIdx.x; i < n; i += kThreads) out[i] = batch[b].logits[i];
+                *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<const uint4*>(batch.logits + i);
+            for (int i = whole + threadIdx.x; i < n; i += kThreads) out[i] = batch.logits[i];
         }
         __syncthreads();   // the batch may be written again
+        fetch_batch(a, first + step, batch);
     }
+    copies_wait<0>();
     if (!a.part) return;
     if (threadIdx.x < kCond) {
         float t = 0.f;
@@ -1150,7 +1172,7 @@ int rl_moves_sample(const void* logits, long long stride, int type, const void* 
     a.dense_logits = dense(logits, stride == kBytes);
     a.dense_masks = dense(masks, mask_stride == kBytes);
     a.dense_u = dense(u, true);
-    const unsigned grid = blocks_for(rows, kThreads, 6ll * sm_count());
+    const unsigned grid = blocks_for(rows, kThreads, 24ll * sm_count());
     with_type(type, [&](auto t) {
         using T = decltype(t);
         k_moves_sample<T><<<grid, kThreads, 2 * sizeof(MoveBatch<T>), static_cast<cudaStream_t>(stream)>>>(a);
@@ -1220,10 +1242,10 @@ int rl_moves_logp(const void* logits, long long stride, int type, const void* co
     a.rows = rows;
     a.dense_logits = dense(logits, stride == kBytes);
     a.dense_masks = dense(masks, mask_stride == kBytes);
-    const unsigned grid = blocks_for(rows, kThreads, 8ll * sm_count());
+    const unsigned grid = blocks_for(rows, kThreads, 24ll * sm_count());
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        k_moves_logp<T><<<grid, kThreads, 2 * sizeof(LogpBatch<T>), static_cast<cudaStream_t>(stream)>>>(a);
+        k_moves_logp<T><<<grid, kThreads, 2 * sizeof(LogpBatch<T, kThreads>), static_cast<cudaStream_t>(stream)>>>(a);
     });
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? 0 : failed(cudaGetErrorString(e));
@@ -1258,12 +1280,12 @@ int rl_moves_logp_bwd(const void* glp, long long glp_stride, const void* gent, l
     a.dense_logits = dense(logits, stride == kBytes);
     a.dense_masks = dense(masks, mask_stride == kBytes);
     a.dense_out = dense(dlogits, true);
-    const unsigned grid = blocks_for(rows, kThreads, static_cast<long long>(kGradBlocks) * sm_count());
+    const unsigned grid = blocks_for(rows, kGradRows * kThreads, static_cast<long long>(kGradBlocks) * sm_count());
     auto s = static_cast<cudaStream_t>(stream);
     cudaError_t e = cudaSuccess;
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        e = launch<k_moves_grad<T>>(grid, 2 * sizeof(LogpBatch<T>) + (dcond ? kGradSums : 0), s, a);
+        e = launch<k_moves_grad<T>>(grid, sizeof(LogpBatch<T, kGradRows * kThreads>) + (dcond ? kGradSums : 0), s, a);
     });
     if (e == cudaSuccess) e = cudaGetLastError();
     if (e == cudaSuccess && dcond) {

@@ -34,7 +34,6 @@ constexpr int kParts = 5, kBytes = 19, kMoves = 324, kTables = 10, kCond = 127;
 constexpr float kScale = 134217728.f;   // 2^27
 constexpr float kUnit = 1.f / kScale;
 constexpr int kThreads = 128;           // and rows of a block's batch
-constexpr int kGradRows = 2;            // rows of a thread at a time in the backward
 constexpr int kDevices = 64;            // whose properties are kept
 constexpr int kMaxWidth = 4096;         // 2^12 weights of 2^27 and a u of 2^24 fit 63 bits
 
@@ -114,21 +113,23 @@ __device__ __forceinline__ unsigned bits24(float u) {
     return static_cast<unsigned>(min(max(v, 0), 0xFFFFFF));
 }
 
-// All ten tables, in fp32, into shared memory: an entry per thread, so that they arrive together.
+// All ten tables, in fp32, into shared memory: an entry per thread (or two), so that they arrive together.
 __device__ __forceinline__ void load_cond(float* tab, const Cond& c) {
-    static_assert(kCond <= kThreads, "an entry per thread");
-    if (c.type < 0 || threadIdx.x >= kCond) return;
-    int t = 0, at = 0;
+    if (c.type < 0) return;
+#pragma unroll 2
+    for (int e = threadIdx.x; e < kCond; e += blockDim.x) {
+        int t = 0, at = 0;
 #pragma unroll
-    for (int i = 1; i < kTables; ++i)
-        if (static_cast<int>(threadIdx.x) >= table_at(i)) {
-            t = i;
-            at = table_at(i);
-        }
-    const int i = static_cast<int>(threadIdx.x) - at;
-    tab[threadIdx.x] = c.type == 0 ? static_cast<const float*>(c.table[t])[i]
-                       : c.type == 1 ? to_f(static_cast<const __nv_bfloat16*>(c.table[t])[i])
-                                     : to_f(static_cast<const __half*>(c.table[t])[i]);
+        for (int i = 1; i < kTables; ++i)
+            if (e >= table_at(i)) {
+                t = i;
+                at = table_at(i);
+            }
+        const int i = e - at;
+        tab[e] = c.type == 0 ? static_cast<const float*>(c.table[t])[i]
+                 : c.type == 1 ? to_f(static_cast<const __nv_bfloat16*>(c.table[t])[i])
+                               : to_f(static_cast<const __half*>(c.table[t])[i]);
+    }
 }
 
 // ------------------------------------------------------------------ batches of rows in shared memory
@@ -146,16 +147,16 @@ template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // Rows [first, first + n) of COLS values each into shared memory, end to end.
-template <int COLS, class T>
+template <int COLS, int THREADS, class T>
 __device__ __forceinline__ void stage(T* dst, const void* base, long long first, int n, long long stride, bool dense) {
     const T* src = static_cast<const T*>(base) + first * stride;
     if (dense) {
         constexpr int kPer = 16 / static_cast<int>(sizeof(T));
         const int all = n * COLS, whole = all & ~(kPer - 1);
-        for (int i = threadIdx.x * kPer; i < whole; i += kThreads * kPer) copy16(dst + i, src + i);
-        for (int i = whole + threadIdx.x; i < all; i += kThreads) dst[i] = src[i];
+        for (int i = threadIdx.x * kPer; i < whole; i += THREADS * kPer) copy16(dst + i, src + i);
+        for (int i = whole + threadIdx.x; i < all; i += THREADS) dst[i] = src[i];
     } else {
-        for (int i = threadIdx.x; i < n * COLS; i += kThreads) {
+        for (int i = threadIdx.x; i < n * COLS; i += THREADS) {
             const int row = i / COLS;
             dst[i] = src[row * stride + (i - row * COLS)];
         }
@@ -310,9 +311,9 @@ __global__ void __launch_bounds__(kThreads) k_moves_sample(MoveArgs a) {
     auto fetch = [&](long long first, MoveBatch<T>& to) {
         if (first < a.rows) {
             const int n = static_cast<int>(min(static_cast<long long>(kThreads), a.rows - first));
-            stage<kBytes>(to.logits, a.logits, first, n, a.stride, a.dense_logits);
-            stage<kBytes>(to.masks, a.masks, first, n, a.mask_stride, a.dense_masks);
-            stage<kParts>(to.u, a.u, first, n, kParts, a.dense_u);
+            stage<kBytes, kThreads>(to.logits, a.logits, first, n, a.stride, a.dense_logits);
+            stage<kBytes, kThreads>(to.masks, a.masks, first, n, a.mask_stride, a.dense_masks);
+            stage<kParts, kThreads>(to.u, a.u, first, n, kParts, a.dense_u);
         }
         copies_commit();
     };
@@ -808,12 +809,12 @@ struct LogpBatch {
     alignas(16) uint8_t masks[ROWS * kBytes];
 };
 
-template <class T, int ROWS>
+template <int THREADS, class T, int ROWS>
 __device__ __forceinline__ void fetch_batch(const LogpArgs& a, long long first, LogpBatch<T, ROWS>& to) {
     if (first < a.rows) {
         const int n = static_cast<int>(min(static_cast<long long>(ROWS), a.rows - first));
-        stage<kBytes>(to.logits, a.logits, first, n, a.stride, a.dense_logits);
-        stage<kBytes>(to.masks, a.masks, first, n, a.mask_stride, a.dense_masks);
+        stage<kBytes, THREADS>(to.logits, a.logits, first, n, a.stride, a.dense_logits);
+        stage<kBytes, THREADS>(to.masks, a.masks, first, n, a.mask_stride, a.dense_masks);
     }
     copies_commit();
 }
@@ -828,8 +829,8 @@ struct SoftRow {
     unsigned some;            // bit k: part k has a legal choice
 };
 
-template <int R, class T>
-__device__ __forceinline__ void soft_rows(SoftRow (&s)[R], const T* const (&logits)[R], const uint8_t* const (&mask)[R], const float* tab,
+template <int R, class P>
+__device__ __forceinline__ void soft_rows(SoftRow (&s)[R], P const (&logits)[R], const uint8_t* const (&mask)[R], const float* tab,
                                           const int (&c)[R][kParts]) {
     float m[R][kParts];
     bool odd = false;
@@ -905,11 +906,11 @@ __global__ void __launch_bounds__(kThreads) k_moves_logp(LogpArgs a) {
     auto* batch = reinterpret_cast<LogpBatch<T, kThreads>*>(batches);
     const long long step = static_cast<long long>(gridDim.x) * kThreads;
     long long first = static_cast<long long>(blockIdx.x) * kThreads;
-    fetch_batch(a, first, batch[0]);
+    fetch_batch<kThreads>(a, first, batch[0]);
     load_cond(tab_s, a.cond);
     const float* tab = a.cond.type < 0 ? nullptr : tab_s;
     for (int b = 0; first < a.rows; first += step, b ^= 1) {
-        fetch_batch(a, first + step, batch[b ^ 1]);
+        fetch_batch<kThreads>(a, first + step, batch[b ^ 1]);
         const long long row = first + threadIdx.x;
         const int id = row < a.rows ? a.ids[row] : 0;
         copies_wait<1>();
@@ -941,23 +942,26 @@ __global__ void __launch_bounds__(kThreads) k_moves_logp(LogpArgs a) {
 // dl = ga 1[i = c] - p (ga + gb (d - mean_d)), in the logits' place in shared memory and from there to memory as one stretch.
 // Every thread sums the tables' gradient in a column of its own of shared memory, so that no two add to one place and the
 // order of the additions is the launch's alone; the 23 additions of a row go to 23 places, so they are read together and
-// written together. The columns' 65 KB leave 8 warps per SM, so a thread takes two rows side by side.
-template <class T>
-__global__ void __launch_bounds__(kThreads) k_moves_grad(LogpArgs a) {
-    extern __shared__ __align__(16) unsigned char batches[];   // a batch, then [127][kThreads] sums
+// written together. The columns' 508 bytes per thread leave 8 to 10 warps per SM, so a thread takes R = 2 rows side by side
+// where there are rows for it (8,192 x 128 rows: 76 us with one row per thread and the next batch on its way, 80 us with two
+// and 256 threads, 70 us with two and 128, 59 us with two and blocks of 64); one row each where every block has one batch
+// at most.
+template <class T, int THREADS, int R>
+__global__ void __launch_bounds__(THREADS) k_moves_grad(LogpArgs a) {
+    extern __shared__ __align__(16) unsigned char batches[];   // a batch, then [127][THREADS] sums
     __shared__ float tab_s[kCond];
     __shared__ uint8_t none_s[kBytes];
-    constexpr int R = kGradRows, kRows = R * kThreads;
+    constexpr int kRows = R * THREADS;
     auto& batch = *reinterpret_cast<LogpBatch<T, kRows>*>(batches);
     float* acc_s = reinterpret_cast<float*>(batches + sizeof(batch));
     const long long step = static_cast<long long>(gridDim.x) * kRows;
     long long first = static_cast<long long>(blockIdx.x) * kRows;
-    fetch_batch(a, first, batch);
+    fetch_batch<THREADS>(a, first, batch);
     if (threadIdx.x < kBytes) none_s[threadIdx.x] = 0;
     load_cond(tab_s, a.cond);
     float* acc = a.part ? acc_s + threadIdx.x : nullptr;
     if (acc)
-        for (int e = 0; e < kCond; ++e) acc[e * kThreads] = 0.f;
+        for (int e = 0; e < kCond; ++e) acc[e * THREADS] = 0.f;
     const float* tab = a.cond.type < 0 ? nullptr : tab_s;
     for (; first < a.rows; first += step) {
         float ga[R], gb[R];
@@ -966,7 +970,7 @@ __global__ void __launch_bounds__(kThreads) k_moves_grad(LogpArgs a) {
         const uint8_t* mask[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const int at = threadIdx.x + r * kThreads;
+            const int at = threadIdx.x + r * THREADS;
             const long long row = first + at;
             ga[r] = gb[r] = 0.f;
             id[r] = -1;
@@ -982,9 +986,7 @@ __global__ void __launch_bounds__(kThreads) k_moves_grad(LogpArgs a) {
         copies_wait<0>();
         __syncthreads();
         SoftRow s[R];
-        const T* const from[R] = {logits[0], logits[1]};
-        const uint8_t* const masks[R] = {mask[0], mask[1]};
-        soft_rows<R>(s, from, masks, tab, c);
+        soft_rows<R>(s, logits, mask, tab, c);
         float g[R][kBytes];
 #pragma unroll
         for (int r = 0; r < R; ++r)
@@ -1011,7 +1013,7 @@ __global__ void __launch_bounds__(kThreads) k_moves_grad(LogpArgs a) {
                     for (int j = 0; j < k; ++j)
 #pragma unroll
                         for (int i = 0; i < part_n(k); ++i)
-                            sum[n++] = acc[(table_at(table_of(k, j)) + c[r][j] * part_n(k) + i) * kThreads] + g[r][part_at(k) + i];
+                            sum[n++] = acc[(table_at(table_of(k, j)) + c[r][j] * part_n(k) + i) * THREADS] + g[r][part_at(k) + i];
                 n = 0;
 #pragma unroll
                 for (int k = 1; k < kParts; ++k)
@@ -1019,7 +1021,7 @@ __global__ void __launch_bounds__(kThreads) k_moves_grad(LogpArgs a) {
                     for (int j = 0; j < k; ++j)
 #pragma unroll
                         for (int i = 0; i < part_n(k); ++i)
-                            acc[(table_at(table_of(k, j)) + c[r][j] * part_n(k) + i) * kThreads] = sum[n++];
+                            acc[(table_at(table_of(k, j)) + c[r][j] * part_n(k) + i) * THREADS] = sum[n++];
             }
 #pragma unroll
             for (int e = 0; e < kBytes; ++e) logits[r][e] = from_f<T>(g[r][e]);
@@ -1030,19 +1032,19 @@ __global__ void __launch_bounds__(kThreads) k_moves_grad(LogpArgs a) {
             T* out = static_cast<T*>(a.dlogits) + first * kBytes;
             constexpr int kPer = 16 / static_cast<int>(sizeof(T));
             const int whole = a.dense_out ? n & ~(kPer - 1) : 0;
-            for (int i = threadIdx.x * kPer; i < whole; i += kThreads * kPer)
+            for (int i = threadIdx.x * kPer; i < whole; i += THREADS * kPer)
                 *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<const uint4*>(batch.logits + i);
-            for (int i = whole + threadIdx.x; i < n; i += kThreads) out[i] = batch.logits[i];
+            for (int i = whole + threadIdx.x; i < n; i += THREADS) out[i] = batch.logits[i];
         }
         __syncthreads();   // the batch may be written again
-        fetch_batch(a, first + step, batch);
+        fetch_batch<THREADS>(a, first + step, batch);
     }
     copies_wait<0>();
     if (!a.part) return;
-    if (threadIdx.x < kCond) {
+    for (int e = threadIdx.x; e < kCond; e += THREADS) {   // each reader starts at a bank of its own
         float t = 0.f;
-        for (int j = 0; j < kThreads; ++j) t += acc_s[threadIdx.x * kThreads + (j + threadIdx.x) % kThreads];
-        a.part[static_cast<long long>(blockIdx.x) * kCond + threadIdx.x] = t;
+        for (int j = 0; j < THREADS; ++j) t += acc_s[e * THREADS + (j + e) % THREADS];
+        a.part[static_cast<long long>(blockIdx.x) * kCond + e] = t;
     }
 }
 
@@ -1055,8 +1057,7 @@ __global__ void __launch_bounds__(32) k_moves_grad_sum(const float* part, int bl
     if (threadIdx.x == 0) dcond[blockIdx.x] = t;
 }
 
-constexpr int kGradBlocks = 2;   // per SM: each has 65 KB of table sums
-constexpr size_t kGradSums = static_cast<size_t>(kCond) * kThreads * sizeof(float);
+constexpr int kGradThreads = 64, kGradBlocks = 5;   // of the backward, and per SM: 32 KB of table sums and 12 KB of rows each
 
 int current_device() {
     int dev = 0;
@@ -1075,19 +1076,20 @@ int sm_count() {
     return sms;
 }
 
-// Launches a kernel that may need more shared memory than the 48 KB it has unasked (asked for once per device).
+// Launches a kernel that may need more shared memory than the 48 KB it has unasked; `most`, the most that it is ever
+// launched with, is asked for once per device.
 template <auto KERNEL, class A>
-cudaError_t launch(unsigned grid, size_t smem, cudaStream_t stream, const A& a) {
+cudaError_t launch(unsigned grid, int block, size_t smem, size_t most, cudaStream_t stream, const A& a) {
     static std::atomic<bool> asked[kDevices];
-    if (smem > 48 * 1024) {
+    if (most > 48 * 1024) {
         const int dev = current_device();
         if (dev < 0 || dev >= kDevices || !asked[dev].load(std::memory_order_acquire)) {
-            const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+            const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
             if (e != cudaSuccess) return e;
             if (dev >= 0 && dev < kDevices) asked[dev].store(true, std::memory_order_release);
         }
     }
-    KERNEL<<<grid, kThreads, smem, stream>>>(a);
+    KERNEL<<<grid, static_cast<unsigned>(block), smem, stream>>>(a);
     return cudaSuccess;
 }
 
@@ -1280,12 +1282,20 @@ int rl_moves_logp_bwd(const void* glp, long long glp_stride, const void* gent, l
     a.dense_logits = dense(logits, stride == kBytes);
     a.dense_masks = dense(masks, mask_stride == kBytes);
     a.dense_out = dense(dlogits, true);
-    const unsigned grid = blocks_for(rows, kGradRows * kThreads, static_cast<long long>(kGradBlocks) * sm_count());
     auto s = static_cast<cudaStream_t>(stream);
     cudaError_t e = cudaSuccess;
+    unsigned grid = 0;
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        e = launch<k_moves_grad<T>>(grid, sizeof(LogpBatch<T, kGradRows * kThreads>) + (dcond ? kGradSums : 0), s, a);
+        auto run = [&](auto per_thread) {
+            constexpr int R = per_thread();
+            constexpr size_t kBatch = sizeof(LogpBatch<T, R * kGradThreads>);
+            constexpr size_t kSums = static_cast<size_t>(kCond) * kGradThreads * sizeof(float);
+            grid = blocks_for(rows, R * kGradThreads, static_cast<long long>(kGradBlocks) * sm_count());
+            e = launch<k_moves_grad<T, kGradThreads, R>>(grid, kGradThreads, dcond ? kBatch + kSums : kBatch, kBatch + kSums, s, a);
+        };
+        if (rows <= static_cast<long long>(kGradBlocks) * kGradThreads * sm_count()) run(std::integral_constant<int, 1>{});
+        else run(std::integral_constant<int, 2>{});
     });
     if (e == cudaSuccess) e = cudaGetLastError();
     if (e == cudaSuccess && dcond) {

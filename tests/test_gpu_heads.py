@@ -532,3 +532,30 @@ def test_c_entry_refusals():
                lib.rl_moves_logp_bwd(one, 1, one, 1, one, 19, 0, None, 0, one, 19, one, one, None, 0, None, 0, None)):
         assert rc != 0 and lib.rl_heads_error()
     assert moves(rows=0) == 0 and rows_(rows=0) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('kind', ['fp32', 'bf16'])
+def test_gradients_of_a_large_batch(lib, kind):
+    """More rows than one batch per block: the logits' gradients first without the tables', then with them, equal row by row
+    to a small batch's; the tables' to (rows / 32 + 64) 2^-24 of the summed terms."""
+    rows = 90001
+    logits, cond, masks, _, g = _inputs(rows, 91, DT[kind], empty=0.01)
+    ids = _legal_ids(masks, g)
+    ga, gb = torch.randn(rows, generator=g), torch.randn(rows, generator=g) * 0.1
+    mc, ic, gc = masks.cuda(), ids.cuda(), (ga.cuda(), gb.cuda())
+    fixed = [q.cuda() for q in cond]
+    a = logits.cuda().requires_grad_(True)
+    alone, = torch.autograd.grad(moves_logp(a, fixed, mc, ic), [a], gc)
+    t = [q.clone().requires_grad_(True) for q in fixed]
+    grads = torch.autograd.grad(moves_logp(a, t, mc, ic), [a, *t], gc)
+    assert torch.equal(grads[0], alone)
+    for lo, hi in ((0, 300), (44000, 44511), (89800, rows)):
+        b = logits[lo:hi].cuda().requires_grad_(True)
+        part, = torch.autograd.grad(moves_logp(b, fixed, mc[lo:hi], ic[lo:hi]), [b], (gc[0][lo:hi], gc[1][lo:hi]))
+        assert torch.equal(part, alone[lo:hi])
+    a64, t64 = logits.double().requires_grad_(True), [q.double().requires_grad_(True) for q in cond]
+    refs = torch.autograd.grad(_logp64(a64, t64, masks, ids), [a64, *t64], (ga.double(), gb.double()))
+    bound = float(((ga.abs() + 20 * gb.abs()).double() * 12 * 17 * U).sum()) + (rows / 32 + 64) * U * rows ** 0.5 * 4
+    for got, ref in zip(grads[1:], refs[1:]):
+        assert float((got.cpu().double() - ref).abs().max()) <= bound

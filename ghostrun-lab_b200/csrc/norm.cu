@@ -5,6 +5,10 @@
 //   h = gy w, dx = r (h - mean(h) - xh mean(h xh)) + gsum, dw = sum over rows of gy xh, db = sum over rows of gy
 // All of it in fp32 from the inputs' types, rounded once into the outputs'. The variance is summed from the centred
 // values (a second pass), so that a large mean costs no digits.
+//
+// Bound by memory: every value is read once and written once (1,048,576 x 512 bf16 with residuals: forward 4.3 GB in 728 us,
+// 5.9 TB/s; backward 4.3 GB in 613 us, 7.0 TB/s; a plain copy 6.5). A warp or a block therefore keeps a row in registers,
+// and the copies of coming rows are under way all the time.
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -22,7 +26,9 @@ constexpr int kWideThreads = 512;
 constexpr int kDevices = 64;                               // whose properties are kept
 constexpr int kMaxRow = 8192;                              // values of a row that a block's registers hold
 constexpr int kCols = 64, kColRows = kThreads / kCols;
-constexpr int kFwdWarps = 16, kBwdWarps = 16;              // warps per SM that share the rows
+// Warps per SM that share the rows (524,288 x 512 bf16 with residuals: 24 warps forward 375 us against 360; 24 backward
+// spill, 418 against 279).
+constexpr int kFwdWarps = 16, kBwdWarps = 16;
 
 thread_local std::string g_norm_error;
 
@@ -701,10 +707,16 @@ cudaError_t launch(unsigned grid, int block, size_t smem, cudaStream_t stream, c
     return cudaSuccess;
 }
 
-int failed(const char* msg) {
-    g_norm_error = msg;
+int failed(const char* msg) noexcept {
+    try {
+        g_norm_error = msg;
+    } catch (...) {   // no memory for the message: the code alone
+    }
     return 1;
 }
+
+// Whether a (non-null) pointer may hold values of a type.
+bool fits(const void* p, int type) { return reinterpret_cast<uintptr_t>(p) % (type == 0 ? 4 : 2) == 0; }
 
 // f of the row's tile (threads per row, values per thread): the smallest that holds it.
 template <class F>
@@ -758,6 +770,9 @@ int rl_norm_fwd(const void* x, const void* residual, const void* weight, const v
     if (const char* e = bad_shape(rows, width, x_type, y_type, w_type)) return failed(e);
     if (rows == 0) return 0;
     if (!x || !y || (residual && !sum)) return failed("x, y and (with a residual) sum must be given");
+    if (!fits(x, x_type) || !fits(residual, x_type) || !fits(y, y_type) || !fits(sum, x_type) || !fits(weight, w_type) ||
+        !fits(bias, w_type) || reinterpret_cast<uintptr_t>(stats) % 8)
+        return failed("misaligned pointer");
     FwdArgs a{x, residual, weight, bias, y, sum, static_cast<float2*>(stats), rows, width, x_stride, r_stride, w_type, aligned(weight, 0, w_type) && aligned(bias, 0, w_type), eps};
     auto s = static_cast<cudaStream_t>(stream);
     cudaError_t e = cudaSuccess;
@@ -795,6 +810,9 @@ int rl_norm_bwd(const void* gy, const void* gsum, const void* s, const void* sta
     if (const char* e = bad_shape(rows, width, x_type, y_type, w_type)) return failed(e);
     if (rows < 1) return failed("rows must be positive");
     if (!gy || !s || !stats) return failed("gy, s and stats must be given");
+    if (!fits(gy, y_type) || !fits(gsum, x_type) || !fits(s, x_type) || !fits(weight, w_type) || !fits(dx, x_type) ||
+        !fits(dweight, w_type) || !fits(dbias, w_type) || !fits(work, 0) || reinterpret_cast<uintptr_t>(stats) % 8)
+        return failed("misaligned pointer");
     const bool params = dweight || dbias;
     if (params && (!work || work_bytes < rl_norm_bwd_work_bytes(rows, width)))
         return failed("work space smaller than rl_norm_bwd_work_bytes()");

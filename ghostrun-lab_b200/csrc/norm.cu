@@ -29,6 +29,9 @@ constexpr int kCols = 64, kColRows = kThreads / kCols;
 // Warps per SM that share the rows (524,288 x 512 bf16 with residuals: 24 warps forward 375 us against 360; 24 backward
 // spill, 418 against 279).
 constexpr int kFwdWarps = 16, kBwdWarps = 16;
+// Rows read value by value have their loads in flight in registers, so 8 values per thread go with more warps (1,048,576 x 201
+// bf16 forward: 452 us with 16, 350 with 24).
+constexpr int kFwdWarpsOne = 24;
 
 thread_local std::string g_norm_error;
 
@@ -224,6 +227,7 @@ constexpr int depth_of(int warps) {
 template <class TX, class TY, bool VEC, int TPR, int EPT>
 struct Fwd : Tile<TX, VEC, TPR, EPT> {
     static constexpr int kW = kWords<TX, VEC, EPT>;
+    static constexpr int kBlocks = (VEC || EPT > 8 ? kFwdWarps : kFwdWarpsOne) * 32 / Fwd::kBlock;   // per SM
     static constexpr int kDepth = depth_of<2 * kW>(kFwdWarps);
     static constexpr size_t kSmem = static_cast<size_t>(kDepth) * 2 * kW * 16 * Fwd::kBlock;
 };
@@ -231,6 +235,7 @@ struct Fwd : Tile<TX, VEC, TPR, EPT> {
 template <class TX, class TY, bool VEC, int TPR, int EPT>
 struct Bwd : Tile<TX, VEC, TPR, EPT> {
     static constexpr int kW = kWords<TX, VEC, EPT>, kG = kWords<TY, VEC, EPT>;
+    static constexpr int kBlocks = kBwdWarps * 32 / Bwd::kBlock;   // per SM
     static constexpr int kDepth = depth_of<2 * kW + kG>(kBwdWarps);
     static constexpr size_t kRing = static_cast<size_t>(kDepth) * (2 * kW + kG) * 16 * Bwd::kBlock;
     static constexpr size_t kCols = 2 * sizeof(float) * EPT * Bwd::kBlock;   // at the end, in the ring's place
@@ -240,7 +245,7 @@ struct Bwd : Tile<TX, VEC, TPR, EPT> {
 // Rows go to teams of TPR threads; the lanes of a warp (teams within one) and the warps of a block (teams of several) take
 // the same number of turns. A team behind the last row works on that row again, and writes nothing.
 template <class TX, class TY, bool VEC, int TPR, int EPT>
-__global__ void __launch_bounds__(Fwd<TX, TY, VEC, TPR, EPT>::kBlock, kFwdWarps * 32 / Fwd<TX, TY, VEC, TPR, EPT>::kBlock)
+__global__ void __launch_bounds__(Fwd<TX, TY, VEC, TPR, EPT>::kBlock, Fwd<TX, TY, VEC, TPR, EPT>::kBlocks)
 k_norm_fwd(FwdArgs a) {
     using L = Fwd<TX, TY, VEC, TPR, EPT>;
     using P = Pack<TX, L::kVe>;
@@ -268,8 +273,27 @@ k_norm_fwd(FwdArgs a) {
             copies_commit();
         }
     };
+    P next_x[VEC ? 1 : NV], next_r[VEC ? 1 : NV];
+    auto load_next = [&](long long at_row) {   // value by value: the next row's loads are under way in registers
+        if constexpr (!VEC) {
+            const long long from = at_row < a.rows ? at_row : a.rows - 1;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                next_x[v] = P{};
+                if (L::at(v, t) < width) next_x[v] = load_pack<TX, E>(static_cast<const TX*>(a.x) + from * a.x_stride + L::at(v, t));
+            }
+            if (a.res) {
+#pragma unroll
+                for (int v = 0; v < NV; ++v) {
+                    next_r[v] = P{};
+                    if (L::at(v, t) < width) next_r[v] = load_pack<TX, E>(static_cast<const TX*>(a.res) + from * a.r_stride + L::at(v, t));
+                }
+            }
+        }
+    };
 #pragma unroll
     for (int q = 0; q < S; ++q) fetch(row + q * step, q);
+    load_next(row);
     float w[EPT], b[EPT];   // behind the first rows' copies, which take as long
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -278,25 +302,26 @@ k_norm_fwd(FwdArgs a) {
     }
     for (int slot = 0; first < a.rows; first += step, row += step) {
         const bool live = row < a.rows;
-        const long long from = live ? row : a.rows - 1;
         if constexpr (VEC) copies_wait<S - 1>();
         P x[NV];
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            x[v] = P{};
-            if (L::at(v, t) < width) {
-                if constexpr (VEC) x[v] = slot_pack<TX, E, B>(ring + (slot * 2 * W + v * (W / NV)) * B + threadIdx.x);
-                else x[v] = load_pack<TX, E>(static_cast<const TX*>(a.x) + from * a.x_stride + L::at(v, t));
+            if constexpr (VEC) {
+                x[v] = P{};
+                if (L::at(v, t) < width) x[v] = slot_pack<TX, E, B>(ring + (slot * 2 * W + v * (W / NV)) * B + threadIdx.x);
+            } else {
+                x[v] = next_x[v];
             }
         }
         if (a.res) {
             P r[NV];
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
-                r[v] = P{};
-                if (L::at(v, t) < width) {
-                    if constexpr (VEC) r[v] = slot_pack<TX, E, B>(ring + (slot * 2 * W + W + v * (W / NV)) * B + threadIdx.x);
-                    else r[v] = load_pack<TX, E>(static_cast<const TX*>(a.res) + from * a.r_stride + L::at(v, t));
+                if constexpr (VEC) {
+                    r[v] = P{};
+                    if (L::at(v, t) < width) r[v] = slot_pack<TX, E, B>(ring + (slot * 2 * W + W + v * (W / NV)) * B + threadIdx.x);
+                } else {
+                    r[v] = next_r[v];
                 }
             }
             TX* ps = static_cast<TX*>(a.sum) + row * width;
@@ -312,6 +337,8 @@ k_norm_fwd(FwdArgs a) {
         if constexpr (VEC) {
             fetch(row + S * step, slot);
             slot = slot + 1 == S ? 0 : slot + 1;
+        } else {
+            load_next(row + step);
         }
         float s[EPT];
         float sum = 0.f;
@@ -349,7 +376,7 @@ k_norm_fwd(FwdArgs a) {
 // the block writes their sums once, a.splits blocks in all. The row's values are read a second time, from shared memory (or
 // L1), when their means are known, not kept in registers.
 template <class TX, class TY, bool VEC, int TPR, int EPT>
-__global__ void __launch_bounds__(Bwd<TX, TY, VEC, TPR, EPT>::kBlock, kBwdWarps * 32 / Bwd<TX, TY, VEC, TPR, EPT>::kBlock)
+__global__ void __launch_bounds__(Bwd<TX, TY, VEC, TPR, EPT>::kBlock, Bwd<TX, TY, VEC, TPR, EPT>::kBlocks)
 k_norm_bwd(BwdArgs a) {
     using L = Bwd<TX, TY, VEC, TPR, EPT>;
     using PX = Pack<TX, L::kVe>;
@@ -388,52 +415,61 @@ k_norm_bwd(BwdArgs a) {
     for (int v = 0; v < NV; ++v) load_params<E>(w + v * E, a.weight, a.w_type, L::at(v, t), width, a.w_wide, 1.f);
 #pragma unroll
     for (int e = 0; e < EPT; ++e) dw[e] = db[e] = 0.f;
+    PX next_s[VEC ? 1 : NV];
+    PY next_g[VEC ? 1 : NV];
+    auto load_next = [&](long long at_row) {
+        if constexpr (!VEC) {
+            const long long from = at_row < a.rows ? at_row : a.rows - 1;
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+                if (L::at(v, t) < width) {
+                    next_s[v] = load_pack<TX, E>(static_cast<const TX*>(a.s) + from * a.s_stride + L::at(v, t));
+                    next_g[v] = load_pack<TY, E>(static_cast<const TY*>(a.gy) + from * a.gy_stride + L::at(v, t));
+                }
+        }
+    };
+    load_next(row);
     float2 st = a.stats[row < a.rows ? row : a.rows - 1];
     for (int slot = 0; first < a.rows; first += step, row += step) {
         const bool live = row < a.rows;
-        const long long from = live ? row : a.rows - 1;
-        const TX* ps = static_cast<const TX*>(a.s) + from * a.s_stride;
-        const TX* pq = static_cast<const TX*>(a.gsum) + from * a.gsum_stride;
-        const TY* pg = static_cast<const TY*>(a.gy) + from * a.gy_stride;
         const uint4* at = ring + slot * R * B + threadIdx.x;
+        PX now_s[VEC ? 1 : NV];
+        PY now_g[VEC ? 1 : NV];
+        if constexpr (VEC) {
+            copies_wait<S - 1>();
+        } else {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                now_s[v] = next_s[v];
+                now_g[v] = next_g[v];
+            }
+            load_next(row + step);
+        }
         auto value_s = [&](int v) -> PX {
             if constexpr (VEC) return slot_pack<TX, E, B>(at + v * (W / NV) * B);
-            else return load_pack<TX, E>(ps + L::at(v, t));
-        };
-        auto value_q = [&](int v) -> PX {
-            if constexpr (VEC) return slot_pack<TX, E, B>(at + (W + v * (W / NV)) * B);
-            else return load_pack<TX, E>(pq + L::at(v, t));
+            else return now_s[v];
         };
         auto value_g = [&](int v) -> PY {
             if constexpr (VEC) return slot_pack<TY, E, B>(at + (2 * W + v * (G / NV)) * B);
-            else return load_pack<TY, E>(pg + L::at(v, t));
+            else return now_g[v];
         };
-        if constexpr (VEC) copies_wait<S - 1>();
+        auto value_q = [&](int v) -> PX {
+            if constexpr (VEC) return slot_pack<TX, E, B>(at + (W + v * (W / NV)) * B);
+            else return load_pack<TX, E>(static_cast<const TX*>(a.gsum) + row * a.gsum_stride + L::at(v, t));
+        };
         const float mu = st.x, rs = st.y;
         if (row + step < a.rows) st = a.stats[row + step];
         float th = 0.f, thx = 0.f;
         if (live) {
-            PX s[VEC ? 1 : NV];
-            PY g[VEC ? 1 : NV];
-            if constexpr (!VEC) {   // all loads before their first use
-#pragma unroll
-                for (int v = 0; v < NV; ++v)
-                    if (L::at(v, t) < width) {
-                        s[v] = value_s(v);
-                        g[v] = value_g(v);
-                    }
-            }
 #pragma unroll
             for (int v = 0; v < NV; ++v)
                 if (L::at(v, t) < width) {
-                    if constexpr (VEC) {
-                        s[0] = value_s(v);
-                        g[0] = value_g(v);
-                    }
+                    const PX s = value_s(v);
+                    const PY g = value_g(v);
 #pragma unroll
                     for (int i = 0; i < E; ++i) {
                         const int e = v * E + i;
-                        const float q = to_f(g[VEC ? 0 : v].v[i]), xh = (to_f(s[VEC ? 0 : v].v[i]) - mu) * rs, h = q * w[e];
+                        const float q = to_f(g.v[i]), xh = (to_f(s.v[i]) - mu) * rs, h = q * w[e];
                         dw[e] = fmaf(q, xh, dw[e]);
                         db[e] += q;
                         th += h;
@@ -667,20 +703,41 @@ int sm_count() {
     return sms;
 }
 
-// Rows that a block takes at a time.
-int block_rows(long long width) { return width <= 64 ? 32 : width <= 128 ? 16 : width <= 512 ? 8 : width <= 1024 ? 4 : width <= 2048 ? 2 : 1; }
-int block_warps(long long width) { return width <= 4096 ? 8 : 16; }
+// f(threads per row, values per thread) of the tile that holds a row of at most kMaxRow values, the smallest. few: 8 values per
+// thread, for the backward of rows read value by value (262,144 x 1,001 bf16: 885 us with 16 read twice, 500 with 8 kept).
+template <class F>
+void with_tile(long long width, bool few, F f) {
+    using std::integral_constant;
+    if (width <= 64) f(integral_constant<int, 8>{}, integral_constant<int, 8>{});
+    else if (width <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+    else if (width <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+    else if (width > 4096) f(integral_constant<int, 512>{}, integral_constant<int, 16>{});
+    else if (few) {
+        if (width <= 512) f(integral_constant<int, 64>{}, integral_constant<int, 8>{});
+        else if (width <= 1024) f(integral_constant<int, 128>{}, integral_constant<int, 8>{});
+        else if (width <= 2048) f(integral_constant<int, 256>{}, integral_constant<int, 8>{});
+        else f(integral_constant<int, 512>{}, integral_constant<int, 8>{});
+    } else if (width <= 512) f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+    else if (width <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
+    else if (width <= 2048) f(integral_constant<int, 128>{}, integral_constant<int, 16>{});
+    else f(integral_constant<int, 256>{}, integral_constant<int, 16>{});
+}
+
+long long ceil_of(long long a, long long b) { return (a + b - 1) / b; }
 
 // Partial sums of the parameters' gradients: blocks of k_norm_bwd, or row splits of k_norm_dw_wide.
-int splits_of(long long rows, long long width) {
-    long long n, most;
+int splits_of(long long rows, long long width, bool vec) {
+    long long n = 1, most = 1;
     if (width <= kMaxRow) {
-        n = static_cast<long long>(kBwdWarps / block_warps(width)) * sm_count();
-        most = (rows + block_rows(width) - 1) / block_rows(width);
+        with_tile(width, !vec, [&](auto tpr, auto ept) {   // neither depends on the types
+            using V = Bwd<float, float, true, tpr(), ept()>;
+            using N = Bwd<float, float, false, tpr(), ept()>;
+            n = static_cast<long long>(vec ? V::kBlocks : N::kBlocks) * sm_count();
+            most = ceil_of(rows, vec ? V::kRows : N::kRows);
+        });
     } else {
-        const long long blocks = (width + kCols - 1) / kCols;
-        n = (8ll * sm_count() + blocks - 1) / blocks;
-        most = (rows + 16 * kColRows - 1) / (16 * kColRows);
+        n = ceil_of(8ll * sm_count(), ceil_of(width, kCols));
+        most = ceil_of(rows, 16 * kColRows);
     }
     if (n > most) n = most;
     return static_cast<int>(n < 1 ? 1 : n);
@@ -717,20 +774,6 @@ int failed(const char* msg) noexcept {
 
 // Whether a (non-null) pointer may hold values of a type.
 bool fits(const void* p, int type) { return reinterpret_cast<uintptr_t>(p) % (type == 0 ? 4 : 2) == 0; }
-
-// f of the row's tile (threads per row, values per thread): the smallest that holds it.
-template <class F>
-void with_tile(long long width, F f) {
-    using std::integral_constant;
-    if (width <= 64) f(integral_constant<int, 8>{}, integral_constant<int, 8>{});
-    else if (width <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
-    else if (width <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
-    else if (width <= 512) f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
-    else if (width <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
-    else if (width <= 2048) f(integral_constant<int, 128>{}, integral_constant<int, 16>{});
-    else if (width <= 4096) f(integral_constant<int, 256>{}, integral_constant<int, 16>{});
-    else f(integral_constant<int, 512>{}, integral_constant<int, 16>{});
-}
 
 bool aligned(const void* p, long long stride, int type) {
     const long long e = type == 0 ? 4 : 2;
@@ -787,12 +830,15 @@ int rl_norm_fwd(const void* x, const void* residual, const void* weight, const v
             else k_norm_fwd_wide<TX, TY, 1><<<blocks_of(rows, 4), kWideThreads, 0, s>>>(a);
             return;
         }
-        const unsigned grid = blocks_of((rows + block_rows(width) - 1) / block_rows(width), kFwdWarps / block_warps(width));
-        with_tile(width, [&](auto tpr, auto ept) {
-            using V = Fwd<TX, TY, true, tpr(), ept()>;
-            using N = Fwd<TX, TY, false, tpr(), ept()>;
-            e = vec ? launch<k_norm_fwd<TX, TY, true, tpr(), ept()>>(grid, V::kBlock, V::kSmem, s, a)
-                    : launch<k_norm_fwd<TX, TY, false, tpr(), ept()>>(grid, N::kBlock, N::kSmem, s, a);
+        with_tile(width, false, [&](auto tpr, auto ept) {
+            auto run = [&](auto wide) {
+                using K = Fwd<TX, TY, wide(), tpr(), ept()>;
+                e = launch<k_norm_fwd<TX, TY, wide(), tpr(), ept()>>(blocks_of(ceil_of(rows, K::kRows), K::kBlocks), K::kBlock, K::kSmem, s, a);
+            };
+            if constexpr (ept() == 16 || tpr() <= 32) {
+                if (vec) run(std::true_type{});
+                else run(std::false_type{});
+            }
         });
     });
     if (e == cudaSuccess) e = cudaGetLastError();
@@ -801,7 +847,8 @@ int rl_norm_fwd(const void* x, const void* residual, const void* weight, const v
 
 size_t rl_norm_bwd_work_bytes(long long rows, long long width) {
     if (rows < 1 || width < 1) return 0;
-    return static_cast<size_t>(splits_of(rows, width)) * 2 * static_cast<size_t>(width) * sizeof(float);
+    const int one = splits_of(rows, width, false), wide = splits_of(rows, width, true);   // which one depends on the pointers
+    return static_cast<size_t>(one > wide ? one : wide) * 2 * static_cast<size_t>(width) * sizeof(float);
 }
 
 int rl_norm_bwd(const void* gy, const void* gsum, const void* s, const void* stats, const void* weight, void* dx,
@@ -818,7 +865,7 @@ int rl_norm_bwd(const void* gy, const void* gsum, const void* s, const void* sta
         return failed("work space smaller than rl_norm_bwd_work_bytes()");
     BwdArgs a{gy, gsum, s, weight, static_cast<const float2*>(stats), dx, dweight, dbias,
               params ? static_cast<float*>(work) : nullptr, rows, width, gy_stride, gsum_stride, s_stride, w_type,
-              aligned(weight, 0, w_type), splits_of(rows, width)};
+              aligned(weight, 0, w_type), splits_of(rows, width, true)};
     if (!dx && !params) return 0;
     auto q = static_cast<cudaStream_t>(stream);
     cudaError_t e = cudaSuccess;
@@ -837,12 +884,16 @@ int rl_norm_bwd(const void* gy, const void* gsum, const void* s, const void* sta
             }
             return;
         }
-        with_tile(width, [&](auto tpr, auto ept) {
-            using V = Bwd<TX, TY, true, tpr(), ept()>;
-            using N = Bwd<TX, TY, false, tpr(), ept()>;
-            const auto grid = static_cast<unsigned>(a.splits);
-            e = vec ? launch<k_norm_bwd<TX, TY, true, tpr(), ept()>>(grid, V::kBlock, V::kSmem, q, a)
-                    : launch<k_norm_bwd<TX, TY, false, tpr(), ept()>>(grid, N::kBlock, N::kSmem, q, a);
+        a.splits = splits_of(rows, width, vec);
+        with_tile(width, !vec, [&](auto tpr, auto ept) {
+            auto run = [&](auto wide) {
+                using K = Bwd<TX, TY, wide(), tpr(), ept()>;
+                e = launch<k_norm_bwd<TX, TY, wide(), tpr(), ept()>>(static_cast<unsigned>(a.splits), K::kBlock, K::kSmem, q, a);
+            };
+            if constexpr (ept() == 16 || tpr() <= 32) {
+                if (vec) return run(std::true_type{});
+            }
+            if constexpr (ept() == 8 || tpr() == 512) run(std::false_type{});
         });
     });
     if (e == cudaSuccess && params) k_norm_dw_sum<<<static_cast<unsigned>((2 * width + 31) / 32), 1024, 0, q>>>(a);

@@ -304,3 +304,31 @@ def test_c_entry_refusals():
     fwd(width=0)
     assert b'width' in lib.rl_norm_error()
     assert fwd(rows=0) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('kind', ['fp32', 'bf16'])
+def test_gradients_through_views_that_are_not_aligned(lib, kind):
+    """Rows that start one value off a 16-byte boundary, and a row's end inside a vector: the same gradients as from rows that
+    lie end to end, to the tolerance of either."""
+    dt = DT[kind]
+    x, r, w, b, g = _inputs(300, 512, dt, 8)
+    gy, gs = torch.randn(300, 512, generator=g).to(dt), torch.randn(300, 512, generator=g).to(dt)
+
+    def wide(t):
+        big = torch.full((300, 517), float('nan'), dtype=dt, device='cuda')
+        big[:, 1:513] = t.cuda()
+        return big
+
+    bx, br = wide(x).requires_grad_(True), wide(r).requires_grad_(True)
+    p = [t.cuda().requires_grad_(True) for t in (w, b)]
+    out = layer_norm(bx[:, 1:513], *p, residual=br[:, 1:513])
+    got = torch.autograd.grad(out, [bx, br, *p], (wide(gy)[:, 1:513], wide(gs)[:, 1:513]))
+    dx, dw, db, mu, sd, xh, h = _grad_refs(_stream(x, r), w, gy, gs)
+    k, lean = _k(512), 1 + mu.abs() / sd
+    size = h.abs() + h.abs().mean(1, keepdim=True) + (xh.abs() + lean) * (h * xh).abs().mean(1, keepdim=True)
+    tol = UNIT[dt] * dx.abs() + 2 * k * lean * (1 + xh.abs()) * size / sd + 2.0 ** -24
+    for d in got[:2]:
+        assert not ((d[:, 1:513].double().cpu() - dx).abs() > tol).any() and not d[:, 0].any() and not d[:, 513:].any()
+    for d, ref, terms in ((got[2], dw, gy.double().abs() * (xh.abs() + lean)), (got[3], db, gy.double().abs())):
+        assert ((d.double().cpu() - ref).abs() <= 2.0 ** -24 * ref.abs() + (k + (300 / 32 + 64) * 2.0 ** -24) * terms.sum(0)).all()

@@ -42,6 +42,18 @@ __device__ __forceinline__ u64 warp_total(u64 v) {
            (static_cast<u64>(__reduce_add_sync(~0u, static_cast<unsigned>(v >> 16))) << 16);
 }
 
+// The sum of v over the lanes of the warp before this one.
+template <class V>
+__device__ __forceinline__ V lanes_before(V v) {
+    V run = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const V up = __shfl_up_sync(~0u, run, o);
+        if ((threadIdx.x & 31) >= o) run += up;
+    }
+    return run - v;
+}
+
 // Sums and the like over the TPR threads of a row: one warp's by its reduction instructions, more warps' (one row per
 // block) through shared memory, in two places that take turns, so that one barrier per call is enough (integer atomics on
 // one word per call took longer: 80 us against 74 for 2,049 rows of 4,001 with every truncation).
@@ -49,7 +61,7 @@ template <int TPR>
 struct Team {
     static constexpr int kWarps = TPR / 32;
     struct Shared {
-        u64 word[2][2][kWarps], warp[2][kWarps];
+        u64 word[2][2][kWarps], warp[2][kWarps], part[32];
     };
     Shared* s;
     int turn = 0, side = 0;
@@ -104,15 +116,12 @@ struct Team {
         count = static_cast<unsigned>(b);
         return static_cast<unsigned>(a);
     }
+    // 32 words, one use per row.
+    __device__ u64* parts() { return s->part; }
     // The sum of v over the threads before this one.
     template <class V>
     __device__ V before(V v) {
-        V run = v;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const V up = __shfl_up_sync(~0u, run, o);
-            if ((threadIdx.x & 31) >= o) run += up;
-        }
+        V run = lanes_before(v) + v;
         if constexpr (kWarps > 1) {
             u64* p = s->warp[side];
             side ^= 1;
@@ -270,6 +279,157 @@ __device__ __forceinline__ float kth_bound(const RowTile<TPR, EPT>& r, Team<TPR>
     return t > floor + 1 ? value_of(t - 1) : -INFINITY;
 }
 
+constexpr int kFew = 128;   // choices that one warp takes on from a block
+
+// Shared memory of a team: the choices between a cut's ends (32 values, 32 weights), and the ones that top-k left.
+struct Few {
+    uint4 ranked[16];
+    float l[kFew];
+    unsigned wgt[kFew];
+    unsigned short at[kFew];
+    unsigned count[32];   // of each stretch and warp
+};
+
+// Lays the row's choices above -inf, at most kFew, end to end in index order.
+template <int TPR, int EPT>
+__device__ __forceinline__ void gather(const RowTile<TPR, EPT>& r, Team<TPR>&, Few& few) {
+    constexpr int kStretches = EPT / 4, kWarps = TPR / 32;
+    static_assert(kStretches * kWarps <= 32, "a count per lane");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const unsigned before = (1u << lane) - 1u;
+    unsigned rank[kStretches];   // of the thread's first choice among its warp's in the stretch
+#pragma unroll
+    for (int s = 0; s < kStretches; ++s) {
+        unsigned all = 0;
+        rank[s] = 0;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const unsigned in = __ballot_sync(~0u, r.l[4 * s + p] > -INFINITY);
+            rank[s] += __popc(in & before);
+            all += __popc(in);
+        }
+        if (lane == 0) few.count[s * kWarps + warp] = all;
+    }
+    __syncthreads();
+    const unsigned mine = lane < kStretches * kWarps ? few.count[lane] : 0u;
+    unsigned run = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned up = __shfl_up_sync(~0u, run, o);
+        if (lane >= o) run += up;
+    }
+    run -= mine;
+#pragma unroll
+    for (int s = 0; s < kStretches; ++s) {
+        unsigned place = __shfl_sync(~0u, run, s * kWarps + warp) + rank[s];
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+            if (r.l[4 * s + p] > -INFINITY) {
+                few.l[place] = r.l[4 * s + p];
+                few.wgt[place] = r.wgt[4 * s + p];
+                few.at[place++] = static_cast<unsigned short>(r.at(4 * s + p));
+            }
+    }
+    __syncthreads();
+}
+
+// The rest of a draw from a row whose top-k is done: top-p, min-p, the choice and its log-probability. index(i): which of the
+// row's choices is the i-th here.
+template <int TPR, int EPT, class I>
+__device__ __forceinline__ void finish(RowTile<TPR, EPT>& r, Team<TPR>& team, uint4* few, const RowCut& q, float m, float u, bool nan,
+                                       I index, long long* choice, float* logp) {
+    if (q.top_p < 1.f) {
+        const float floor = m - 20.f / q.scale;   // exp(-20) 2^27 rounds to nothing
+        unsigned w[2] = {0, 0}, count = 0;
+#pragma unroll
+        for (int e = 0; e < EPT; ++e) {
+            w[e / 16] += r.wgt[e];
+            count += r.l[e] > floor;
+        }
+        u64 total;
+        team.sums(EPT > 16 ? static_cast<u64>(w[0]) + w[1] : w[0], count, total, count);
+        const double p = ceil(static_cast<double>(q.top_p) * static_cast<double>(total));
+        const u64 reach = p < 1.0 ? 1ull : static_cast<u64>(p);
+        // choices that could all go together lie below the lowest value that stays: look there first
+        const float least = static_cast<float>(total - reach) * kUnit / static_cast<float>(count);
+        cut_row<true>(r, team, few, reach, m, floor, m + __logf(least) / q.scale, count);
+    }
+    if (q.min_p > 0.f) {
+        const unsigned least = static_cast<unsigned>(ceil(static_cast<double>(q.min_p) * static_cast<double>(kScale)));
+#pragma unroll
+        for (int e = 0; e < EPT; ++e)
+            if (r.wgt[e] < least) r.wgt[e] = 0;
+    }
+    // the stretch of the row, then the thread, then the place in which the running sum passes the target
+    u64 part[EPT / 4], total = 0;
+#pragma unroll
+    for (int s = 0; s < EPT / 4; ++s) part[s] = warp_total(static_cast<u64>(r.wgt[4 * s] + r.wgt[4 * s + 1] + r.wgt[4 * s + 2] + r.wgt[4 * s + 3]));
+    u64 target, skipped = 0;   // skipped: the sum before this warp's part of the stretch
+    int stretch = 0;
+    bool ours = true;          // whether it is this warp's part that the target lies in
+    if constexpr (TPR == 32) {
+#pragma unroll
+        for (int s = 0; s < EPT / 4; ++s) total += part[s];
+        target = (bits24(u) * total) >> 24;
+#pragma unroll
+        for (int s = 0; s + 1 < EPT / 4; ++s)
+            if (stretch == s && target >= skipped + part[s]) {
+                skipped += part[s];
+                stretch = s + 1;
+            }
+    } else {   // a lane per stretch and warp, in index order
+        constexpr int kWarps = TPR / 32, kParts = EPT / 4 * kWarps;
+        static_assert(kParts <= 32, "a part per lane");
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        u64* parts = team.parts();
+        if (lane == 0) {
+#pragma unroll
+            for (int s = 0; s < EPT / 4; ++s) parts[s * kWarps + warp] = part[s];
+        }
+        __syncthreads();
+        u64 run = lane < kParts ? parts[lane] : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 up = __shfl_up_sync(~0u, run, o);
+            if (lane >= o) run += up;
+        }
+        total = __shfl_sync(~0u, run, 31);
+        target = (bits24(u) * total) >> 24;
+        const int at = __ffs(static_cast<int>(__ballot_sync(~0u, run > target))) - 1;   // the first part that passes the target
+        skipped = at > 0 ? __shfl_sync(~0u, run, at - 1) : 0;
+        stretch = at / kWarps;
+        ours = at % kWarps == warp;
+    }
+    if (!ours) return;
+    target -= skipped;
+    unsigned w[4] = {0, 0, 0, 0};
+    float l[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < EPT / 4; ++s)
+        if (stretch == s) {
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                w[p] = r.wgt[4 * s + p];
+                l[p] = r.l[4 * s + p];
+            }
+        }
+    const u64 own = static_cast<u64>(w[0]) + w[1] + w[2] + w[3], run = lanes_before(own);
+    if (run <= target && target < run + own) {
+        unsigned left = static_cast<unsigned>(target - run);
+        int c = 0;
+        float lc = l[0];
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+            if (c == p && left >= w[p]) {
+                left -= w[p];
+                c = p + 1;
+                lc = l[p + 1];
+            }
+        *choice = index(r.at(4 * stretch) + c);
+        *logp = nan ? NAN : (lc - m) * q.scale - logf(static_cast<float>(total) * kUnit);
+    }
+}
+
 // Warps per SM that the registers of EPT choices per thread leave room for.
 template <int EPT>
 constexpr int kRowWarps = EPT <= 4 ? 48 : EPT <= 12 ? 32 : EPT <= 16 ? 24 : 16;
@@ -282,8 +442,8 @@ k_rows_sample(RowArgs a) {
     constexpr int kTeams = TPR == 32 ? 8 : 1;
     __shared__ typename Team<TPR>::Shared team_s;
     Team<TPR> team(&team_s);
-    __shared__ uint4 few_s[kTeams][16];
-    uint4* few = few_s[TPR == 32 ? threadIdx.x >> 5 : 0];
+    __shared__ Few few_s[kTeams];
+    uint4* few = few_s[TPR == 32 ? threadIdx.x >> 5 : 0].ranked;
     const int n = a.width, lane = threadIdx.x & 31;
     const bool parts = a.legal && a.legal_width != n;
     __shared__ uint4 need_s[TPR == 32 && EPT == 12 ? kMoves / 4 : 1];   // the five mask bytes that a packed move needs, as bits
@@ -380,73 +540,36 @@ k_rows_sample(RowArgs a) {
         }
 #pragma unroll
         for (int e = 0; e < EPT; ++e) r.wgt[e] = weight_of((r.l[e] - m) * q.scale);
+        unsigned kept = 0;   // choices before top-k
         if (q.top_k > 0) {
-            unsigned count = 0;
 #pragma unroll
-            for (int e = 0; e < EPT; ++e) count += r.l[e] > -INFINITY;
-            count = team.count(count);
+            for (int e = 0; e < EPT; ++e) kept += r.l[e] > -INFINITY;
+            kept = team.count(kept);
             const unsigned k = static_cast<unsigned>(q.top_k);
-            if (k < count) cut_row<false>(r, team, few, k, m, -INFINITY, kth_bound(r, team, k), count);
+            if (k < kept) cut_row<false>(r, team, few, k, m, -INFINITY, kth_bound(r, team, k), kept);
         }
-        if (q.top_p < 1.f) {
-            const float floor = m - 20.f / q.scale;   // exp(-20) 2^27 rounds to nothing
-            unsigned w[2] = {0, 0}, count = 0;
+        // what a small k left of a wide row is one warp's work (2,049 x 4,001 with every truncation: 64 us without, 56 with it;
+        // without a top-p to follow it does not pay, 34 us against 40)
+        if constexpr (TPR > 32) {
+            if (q.top_p < 1.f && q.top_k > 0 && q.top_k <= kFew && kept > static_cast<unsigned>(q.top_k)) {
+                gather(r, team, few_s[0]);
+                if (threadIdx.x < 32) {
+                    RowTile<32, kFew / 32> f;
 #pragma unroll
-            for (int e = 0; e < EPT; ++e) {
-                w[e / 16] += r.wgt[e];
-                count += r.l[e] > floor;
-            }
-            u64 total;
-            team.sums(EPT > 16 ? static_cast<u64>(w[0]) + w[1] : w[0], count, total, count);
-            const double p = ceil(static_cast<double>(q.top_p) * static_cast<double>(total));
-            const u64 reach = p < 1.0 ? 1ull : static_cast<u64>(p);
-            // choices that could all go together lie below the lowest value that stays: look there first
-            const float least = static_cast<float>(total - reach) * kUnit / static_cast<float>(count);
-            cut_row<true>(r, team, few, reach, m, floor, m + __logf(least) / q.scale, count);
-        }
-        if (q.min_p > 0.f) {
-            const unsigned least = static_cast<unsigned>(ceil(static_cast<double>(q.min_p) * static_cast<double>(kScale)));
-#pragma unroll
-            for (int e = 0; e < EPT; ++e)
-                if (r.wgt[e] < least) r.wgt[e] = 0;
-        }
-        // the stretch of the row, then the thread, then the place in which the running sum passes the target
-        u64 part[EPT / 4], total = 0;
-#pragma unroll
-        for (int s = 0; s < EPT / 4; ++s) {
-            part[s] = team.sum(r.wgt[4 * s] + r.wgt[4 * s + 1] + r.wgt[4 * s + 2] + r.wgt[4 * s + 3]);
-            total += part[s];
-        }
-        u64 target = (bits24(u) * total) >> 24;
-        int stretch = 0;
-        unsigned w[4] = {r.wgt[0], r.wgt[1], r.wgt[2], r.wgt[3]};
-        float l[4] = {r.l[0], r.l[1], r.l[2], r.l[3]};
-#pragma unroll
-        for (int s = 1; s < EPT / 4; ++s)
-            if (stretch == s - 1 && target >= part[s - 1]) {
-                target -= part[s - 1];
-                stretch = s;
-#pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    w[p] = r.wgt[4 * s + p];
-                    l[p] = r.l[4 * s + p];
+                    for (int e = 0; e < kFew / 32; ++e) {
+                        const bool in = f.at(e) < q.top_k;
+                        f.l[e] = in ? few_s[0].l[f.at(e)] : -INFINITY;
+                        f.wgt[e] = in ? few_s[0].wgt[f.at(e)] : 0u;
+                    }
+                    __syncwarp();   // the gathered values are free, their places are not
+                    Team<32> warp(nullptr);
+                    finish(f, warp, few, q, m, u, nans != 0, [&](int i) { return static_cast<int>(few_s[0].at[i]); }, a.choice + row, a.logp + row);
                 }
+                __syncthreads();
+                continue;
             }
-        const u64 own = static_cast<u64>(w[0]) + w[1] + w[2] + w[3], run = team.before(own);
-        if (run <= target && target < run + own) {
-            unsigned left = static_cast<unsigned>(target - run);
-            int c = 0;
-            float lc = l[0];
-#pragma unroll
-            for (int p = 0; p < 3; ++p)
-                if (c == p && left >= w[p]) {
-                    left -= w[p];
-                    c = p + 1;
-                    lc = l[p + 1];
-                }
-            a.choice[row] = r.at(4 * stretch) + c;
-            a.logp[row] = nans ? NAN : (lc - m) * q.scale - logf(static_cast<float>(total) * kUnit);
         }
+        finish(r, team, few, q, m, u, nans != 0, [](int i) { return i; }, a.choice + row, a.logp + row);
     }
 }
 

@@ -106,13 +106,15 @@ __device__ __forceinline__ float warp_sum(float v) {
 // TPR threads share a row, EPT values each, in vectors of 16 bytes (VEC) or one by one: vector v of thread t starts at
 // value (v TPR + t) VE. A block of 256 threads (512 for the widest rows) takes 256 / TPR rows at a time and goes on to the
 // next ones, whose values are on their way to shared memory meanwhile; the weights stay in registers. Rows that are not
-// 16-byte aligned are read one value at a time, as they are needed.
+// 16-byte aligned are read one value at a time, the next row's into registers.
+
+__host__ __device__ constexpr int block_of(int tpr) { return tpr > kThreads ? tpr : kThreads; }
 
 template <class TX, bool VEC, int TPR, int EPT>
 struct Tile {
     static constexpr int kVe = VEC ? 16 / static_cast<int>(sizeof(TX)) : 1;   // values of a vector
     static constexpr int kNv = EPT / kVe;                                     // vectors of a thread
-    static constexpr int kBlock = TPR > kThreads ? TPR : kThreads;
+    static constexpr int kBlock = block_of(TPR);
     static constexpr int kRows = kBlock / TPR;                                // rows of a block
     static_assert(kNv * kVe == EPT && kRows * TPR == kBlock, "whole vectors, whole rows");
     __device__ static int at(int v, int t) { return (v * TPR + t) * kVe; }
@@ -729,11 +731,9 @@ long long ceil_of(long long a, long long b) { return (a + b - 1) / b; }
 int splits_of(long long rows, long long width, bool vec) {
     long long n = 1, most = 1;
     if (width <= kMaxRow) {
-        with_tile(width, !vec, [&](auto tpr, auto ept) {   // neither depends on the types
-            using V = Bwd<float, float, true, tpr(), ept()>;
-            using N = Bwd<float, float, false, tpr(), ept()>;
-            n = static_cast<long long>(vec ? V::kBlocks : N::kBlocks) * sm_count();
-            most = ceil_of(rows, vec ? V::kRows : N::kRows);
+        with_tile(width, !vec, [&](auto tpr, auto) {
+            n = static_cast<long long>(kBwdWarps * 32 / block_of(tpr())) * sm_count();
+            most = ceil_of(rows, block_of(tpr()) / tpr());
         });
     } else {
         n = ceil_of(8ll * sm_count(), ceil_of(width, kCols));

@@ -65,6 +65,7 @@ const void* at_or_null(const MaybeTensor& t) { return t ? t->const_data_ptr() : 
 void* out_or_null(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 
 Tensor make(at::IntArrayRef shape, at::ScalarType type, const Tensor& like) {
+    const at::AutoDispatchBelowADInplaceOrView below;   // a new tensor has no history to keep
     return at::empty(shape, like.options().dtype(type).memory_format(at::MemoryFormat::Contiguous));
 }
 
@@ -358,6 +359,10 @@ struct MovesLogp : torch::autograd::Function<MovesLogp> {
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        return without_graph(gradients(ctx, std::move(grads)), "moves_logp");
+    }
+
+    static variable_list gradients(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const Tensor &logits = saved[0], &masks = saved[1], &ids = saved[2];
         const at::ArrayRef<Tensor> cond = at::ArrayRef<Tensor>(saved).slice(3);
@@ -387,6 +392,8 @@ struct MovesLogp : torch::autograd::Function<MovesLogp> {
             TORCH_CHECK(rc == 0, "rl_moves_logp_bwd: ", lib.heads_error());
         }
         variable_list out{dlogits, Tensor(), Tensor()};
+        out.reserve(3 + cond.size());
+        const at::AutoDispatchBelowADInplaceOrView below;   // the tables' gradients are parts of one tensor of our own
         int64_t at = 0;
         if (need_cond && cond[0].scalar_type() != at::kFloat) dcond = dcond.to(cond[0].scalar_type());
         for (size_t t = 0; t < cond.size(); ++t) {
@@ -394,7 +401,7 @@ struct MovesLogp : torch::autograd::Function<MovesLogp> {
             out.push_back(ctx->needs_input_grad(3 + t) ? dcond.as_strided({a, b}, {b, 1}, at) : Tensor());
             at += a * b;
         }
-        return without_graph(std::move(out), "moves_logp");
+        return out;
     }
 };
 

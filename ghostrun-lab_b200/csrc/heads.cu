@@ -134,7 +134,7 @@ __device__ __forceinline__ int choose(float (&l)[N], const uint8_t* mask, float 
         d[i] = (l[i] - m) * q.scale;
         w[i] = weight_of(d[i]);
     }
-    if (q.cut) {
+    if (q.cut) {   // (each pair compared once for both its ranks and sums: no faster, and 72 registers instead of 56)
         int rank[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -151,14 +151,13 @@ __device__ __forceinline__ int choose(float (&l)[N], const uint8_t* mask, float 
             total += w[i];
         }
         const unsigned reach = static_cast<unsigned>(ceil(static_cast<double>(q.top_p) * static_cast<double>(total)));
-        const unsigned least = static_cast<unsigned>(ceil(static_cast<double>(q.min_p) * static_cast<double>(kScale)));
         unsigned kept = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             unsigned before = 0;
 #pragma unroll
             for (int j = 0; j < N; ++j) before += rank[j] < rank[i] ? w[j] : 0u;
-            const bool keep = rank[i] == 0 || (before < reach && w[i] >= least);
+            const bool keep = rank[i] == 0 || (before < reach && w[i] >= q.least);
             kept |= static_cast<unsigned>(keep) << i;
         }
 #pragma unroll

@@ -46,27 +46,28 @@ struct Cut {
 };
 
 struct RowCut {
-    float scale;   // 1 / T
-    float top_p, min_p;
-    int top_k;     // 0: all
-    bool cut;      // whether any of the three takes something off
+    float scale;      // 1 / T
+    float top_p;
+    unsigned least;   // min_p 2^27: the least weight that stays
+    int top_k;        // 0: all
+    bool cut;         // whether any of the three takes something off
 };
 
 __device__ __forceinline__ RowCut row_cut(const Cut& c, long long row) {
     RowCut r;
     const float t = c.temperatures ? c.temperatures[row] : c.temperature;
     r.top_p = c.top_ps ? c.top_ps[row] : c.top_p;
-    r.min_p = c.min_ps ? c.min_ps[row] : c.min_p;
+    const float min_p = c.min_ps ? c.min_ps[row] : c.min_p;
     r.top_k = c.top_ks ? c.top_ks[row] : c.top_k;
     r.top_p = r.top_p < 1.f ? fmaxf(r.top_p, 0.f) : 1.f;   // a NaN takes nothing off
-    r.min_p = r.min_p > 0.f ? fminf(r.min_p, 1.f) : 0.f;
+    r.least = min_p > 0.f ? static_cast<unsigned>(ceil(static_cast<double>(fminf(min_p, 1.f)) * static_cast<double>(kScale))) : 0u;
     if (r.top_k < 0) r.top_k = 0;
     r.scale = __fdiv_rn(1.f, t);
     if (!(t > 0.f) || r.scale == INFINITY) {   // 0 (or nothing a temperature can be): the best choice alone
         r.top_k = 1;
         r.scale = 1.f;
     }
-    r.cut = r.top_k > 0 || r.top_p < 1.f || r.min_p > 0.f;
+    r.cut = r.top_k > 0 || r.top_p < 1.f || r.least > 0;
     return r;
 }
 

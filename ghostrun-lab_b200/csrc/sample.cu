@@ -354,11 +354,10 @@ __device__ __forceinline__ void finish(RowTile<TPR, EPT>& r, Team<TPR>& team, ui
         const float least = static_cast<float>(total - reach) * kUnit / static_cast<float>(count);
         cut_row<true>(r, team, few, reach, m, floor, m + __logf(least) / q.scale, count);
     }
-    if (q.min_p > 0.f) {
-        const unsigned least = static_cast<unsigned>(ceil(static_cast<double>(q.min_p) * static_cast<double>(kScale)));
+    if (q.least > 0) {
 #pragma unroll
         for (int e = 0; e < EPT; ++e)
-            if (r.wgt[e] < least) r.wgt[e] = 0;
+            if (r.wgt[e] < q.least) r.wgt[e] = 0;
     }
     // the stretch of the row, then the thread, then the place in which the running sum passes the target
     u64 part[EPT / 4], total = 0;

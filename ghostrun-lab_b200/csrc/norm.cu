@@ -6,8 +6,8 @@
 // All of it in fp32 from the inputs' types, rounded once into the outputs'. The variance is summed from the centred
 // values (a second pass), so that a large mean costs no digits.
 //
-// Bound by memory: every value is read once and written once (1,048,576 x 512 bf16 with residuals: forward 4.3 GB in 728 us,
-// 5.9 TB/s; backward 4.3 GB in 613 us, 7.0 TB/s; a plain copy 6.5). A warp or a block therefore keeps a row in registers,
+// Bound by memory: every value is read once and written once (1,048,576 x 512 bf16 with residuals: forward 4.3 GB in 703 us,
+// 6.1 TB/s; backward 4.3 GB in 609 us, 7.1 TB/s; a plain copy 6.5). A warp or a block therefore keeps a row in registers,
 // and the copies of coming rows are under way all the time.
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>

@@ -18,7 +18,10 @@ def load(path=None):
     """The library, with the C-ABI's argument types, bound to policy_ops_b200; another path takes the place of the one before."""
     global _LIB
     if _LIB is None or path is not None:
-        import policy_ops_b200
+        try:
+            import policy_ops_b200
+        except ImportError as e:
+            raise RuntimeError(f'policy_ops_b200 cannot be loaded ({e}): build it with ghostrun-lab_b200/build.py') from e
         lib = ctypes.CDLL(str(path or default_lib()))
         P, I, L, SZ, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_size_t, ctypes.c_float
         cut = [F, I, F, F, P, P, P, P]

@@ -559,3 +559,35 @@ def test_gradients_of_a_large_batch(lib, kind):
     bound = float(((ga.abs() + 20 * gb.abs()).double() * 12 * 17 * U).sum()) + (rows / 32 + 64) * U * rows ** 0.5 * 4
     for got, ref in zip(grads[1:], refs[1:]):
         assert float((got.cpu().double() - ref).abs().max()) <= bound
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(lib):
+    """113,100,000 rows of 19 and 6,630,000 rows of 324 are more than 2^31 values: their last rows are those of a batch of their
+    own, bit for bit, forward and backward."""
+    g = torch.Generator(device='cuda').manual_seed(3)
+    rows = 113_100_000
+    cond = [torch.randn(s, generator=g, device='cuda') for s in TABLES]
+    logits = torch.randn(rows, 19, generator=g, device='cuda', dtype=torch.bfloat16).requires_grad_(True)
+    masks = torch.randint(0, 2, (rows, 19), generator=g, device='cuda', dtype=torch.uint8)
+    u = torch.rand(rows, 5, generator=g, device='cuda')
+    ids, logp = sample_moves(logits.detach(), cond, masks, u, top_k=4)
+    cut = slice(rows - 2000, rows)
+    few = sample_moves(logits.detach()[cut].clone(), cond, masks[cut].clone(), u[cut].clone(), top_k=4)
+    assert torch.equal(ids[cut], few[0]) and torch.equal(logp[cut], few[1])
+    lp, ent = moves_logp(logits, cond, masks, ids)
+    one = torch.ones(1, device='cuda').expand(rows)
+    d, = torch.autograd.grad((lp, ent), [logits], (one, one))
+    t = logits.detach()[cut].clone().requires_grad_(True)
+    lt, et = moves_logp(t, cond, masks[cut].clone(), ids[cut].clone())
+    assert torch.equal(lp[cut], lt) and torch.equal(ent[cut], et)
+    assert torch.equal(d[cut], torch.autograd.grad((lt, et), [t], (one[cut], one[cut]))[0])
+    del logits, masks, u, ids, logp, lp, ent, d
+    rows = 6_630_000
+    cut = slice(rows - 2000, rows)
+    logits = torch.randn(rows, 324, generator=g, device='cuda', dtype=torch.bfloat16)
+    masks = torch.randint(0, 2, (rows, 19), generator=g, device='cuda', dtype=torch.uint8)
+    u = torch.rand(rows, generator=g, device='cuda')
+    c, p = sample(logits, u, masks, top_p=0.9)
+    few = sample(logits[cut].clone(), u[cut].clone(), masks[cut].clone(), top_p=0.9)
+    assert torch.equal(c[cut], few[0]) and torch.equal(p[cut], few[1])

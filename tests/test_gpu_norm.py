@@ -332,3 +332,22 @@ def test_gradients_through_views_that_are_not_aligned(lib, kind):
         assert not ((d[:, 1:513].double().cpu() - dx).abs() > tol).any() and not d[:, 0].any() and not d[:, 513:].any()
     for d, ref, terms in ((got[2], dw, gy.double().abs() * (xh.abs() + lean)), (got[3], db, gy.double().abs())):
         assert ((d.double().cpu() - ref).abs() <= 2.0 ** -24 * ref.abs() + (k + (300 / 32 + 64) * 2.0 ** -24) * terms.sum(0)).all()
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(lib):
+    """4,200,000 x 512 values are more than 2^31: the last rows, forward and backward, are those of a batch of their own, bit for
+    bit, and the column sums of gradients of 1 are the row count."""
+    rows = 4_200_000
+    g = torch.Generator(device='cuda').manual_seed(12)
+    x = torch.randn(rows, 512, generator=g, device='cuda', dtype=torch.bfloat16).requires_grad_(True)
+    w = (1 + 0.1 * torch.randn(512, generator=g, device='cuda')).requires_grad_(True)
+    b = torch.randn(512, generator=g, device='cuda').requires_grad_(True)
+    y = layer_norm(x, w, b)
+    gy = torch.ones(512, device='cuda', dtype=torch.bfloat16).expand(rows, 512)
+    dx, _, db = torch.autograd.grad(y, (x, w, b), gy)
+    tail = x.detach()[-1000:].clone().requires_grad_(True)
+    yt = layer_norm(tail, w, b)
+    assert torch.equal(y[-1000:], yt)
+    assert torch.equal(dx[-1000:], torch.autograd.grad(yt, tail, gy[-1000:])[0])
+    assert torch.equal(db, torch.full((512,), float(rows), device='cuda'))   # whole numbers below 2^24

@@ -13,8 +13,9 @@ legal is [B, V], or the 19 mask bytes for a flat head over the 324 packed moves,
 temperature (0: the best choice), top_k (0: all), top_p and min_p are numbers, or tensors with one for each row. They apply
 in this order: top-k of the logits / temperature, the shortest run of what is left that holds top_p of its probability,
 those of it with at least min_p of the best one's. Equal logits rank by index. The log-probability returned is that of the
-distribution drawn from. The same inputs give the same choice on any launch shape (csrc/heads.cu). A part (or row) with
-nothing legal answers 0, the neutral choice, with log-probability and entropy 0 and no gradient."""
+distribution drawn from. The same inputs give the same choice on any launch shape (csrc/heads.cuh). The samplers'
+log-probabilities carry no gradient: moves_logp gives the moves' own. A part (or row) with nothing legal answers 0, the neutral
+choice, with log-probability and entropy 0 and no gradient."""
 from __future__ import annotations
 
 import policy_ops

@@ -339,7 +339,9 @@ template <int TPR, int EPT, class I>
 __device__ __forceinline__ void finish(RowTile<TPR, EPT>& r, Team<TPR>& team, uint4* few, const RowCut& q, float m, float u, bool nan,
                                        I index, long long* choice, float* logp) {
     if (q.top_p < 1.f) {
-        const float floor = m - 20.f / q.scale;   // exp(-20) 2^27 rounds to nothing
+        // what weighs nothing lies at floor or below, since exp(-20) 2^27 rounds to 0; one value below m - 20 T as fp32 has it,
+        // which may round up as far as m itself: floor < m always, so the best choice is above it, and so is every weight
+        const float floor = nextafterf(m - 20.f / q.scale, -INFINITY);
         unsigned w[2] = {0, 0}, count = 0;
 #pragma unroll
         for (int e = 0; e < EPT; ++e) {

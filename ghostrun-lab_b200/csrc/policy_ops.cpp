@@ -75,6 +75,15 @@ Tensor rows_of(const Tensor& t, int64_t width) {
     return width == 1 || r.stride(1) == 1 ? r : r.contiguous();
 }
 
+// Forward-mode derivatives are not there: an input that carries one is refused, where the result would be without it.
+void no_tangent(const char* what, const Tensor& t) {
+    TORCH_CHECK(!t._fw_grad(0).defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode(), what,
+                ": an input has a forward-mode derivative, which this operator does not carry");
+}
+void no_tangent(const char* what, const MaybeTensor& t) {
+    if (t) no_tangent(what, *t);
+}
+
 // What a gradient that has no graph of its own is given where the caller keeps one (create_graph): the error comes when a
 // second derivative is asked for.
 variable_list without_graph(variable_list grads, const char* what) {
@@ -198,6 +207,8 @@ py::object layer_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTen
                 residual->sizes(), " ", residual->scalar_type(), " on ", residual->device());
     TORCH_CHECK(out_type == x.scalar_type() || out_type == at::kFloat, "layer_norm: out_dtype must be ", x.scalar_type(),
                 " or fp32, got ", out_type);
+    no_tangent("layer_norm", x);
+    for (const MaybeTensor* t : {&weight, &bias, &residual}) no_tangent("layer_norm", *t);
     const c10::cuda::CUDAGuard guard(x.device());
     Tensor y, sum;
     if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(weight) || wants_grad(bias) || wants_grad(residual))) {
@@ -407,6 +418,9 @@ struct MovesLogp : torch::autograd::Function<MovesLogp> {
 
 py::tuple moves_logp(const Tensor& logits_, const std::optional<std::vector<Tensor>>& cond_, const Tensor& masks_, const Tensor& ids_) {
     const char* what = "moves_logp";
+    no_tangent(what, logits_);
+    if (cond_)
+        for (const Tensor& t : *cond_) no_tangent(what, t);
     const Tensor logits = check_logits(what, logits_, kBytes);
     const c10::cuda::CUDAGuard guard(logits.device());
     const Tensor masks = check_bytes(what, "masks", masks_, logits, kBytes, kBytes);

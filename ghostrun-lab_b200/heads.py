@@ -2,7 +2,7 @@
 entropy of given moves (rl/model.py:176-194, ordered heads masked by the legal parts).
 
     ids, logp = sample_moves(logits, cond, masks, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)
-    logp, entropy = moves_logp(logits, cond, masks, ids)                    # differentiable in logits and cond
+    logp, entropy = moves_logp(logits, cond, masks, ids)                    # differentiable (in reverse) in logits and cond
     choice, logp = sample(logits, u, legal=masks, top_p=0.95)               # rows of any width up to 4096
 
 logits: [B, 19] fp32, bf16 or fp16, the five heads side by side in the mask bytes' order (actions.PARTS); cond: the ten

@@ -6,8 +6,9 @@
 A SimBa block (rl/model.py:64-72) is x + mlp(norm(x)): the sum and the next block's norm read the stream once here. x and
 residual: [..., D] fp32, bf16 or fp16, any leading shape and row strides; weight and bias: [D] of any of the three types,
 each may be None; out_dtype: x's type (default) or fp32. The stream is kept in x's type, and what is kept is what is
-normalised. Statistics and sums are fp32, every output is rounded once. Differentiable (once) in x, residual, weight and
-bias; the gradients of weight and bias are summed in a fixed order, so the same inputs give the same bits."""
+normalised. Statistics and sums are fp32, every output is rounded once. Differentiable (once, in reverse; an input with a
+forward-mode derivative is refused) in x, residual, weight and bias; the gradients of weight and bias are summed in a fixed
+order, so the same inputs give the same bits."""
 from __future__ import annotations
 
 import policy_ops

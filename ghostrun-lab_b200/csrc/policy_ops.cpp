@@ -9,6 +9,7 @@
 #include <torch/extension.h>
 
 #include <cmath>
+#include <limits>
 #include <optional>
 #include <string>
 #include <vector>
@@ -291,7 +292,10 @@ struct Cut {
                                 (i == 1 ? at::isIntegralType(type, false) : at::isIntegralType(type, false) || at::isFloatingType(type)),
                             what, ": ", names[i], " must be a number or [", logits.size(0), "] on ", logits.device(), ", got ", t.sizes(),
                             " ", type, " on ", t.device());
-                each[i] = t.detach().to(i == 1 ? at::kInt : at::kFloat).contiguous();
+                Tensor v = t.detach();
+                if (i == 1 && v.element_size() > 2 && type != at::kInt)   // numbers past 31 bits are no row's width, not their low bits
+                    v = v.to(at::kLong).clamp(0, std::numeric_limits<int>::max());
+                each[i] = v.to(i == 1 ? at::kInt : at::kFloat).contiguous();
             } else {
                 TORCH_CHECK(PyFloat_Check(given[i].ptr()) || PyLong_Check(given[i].ptr()) || PyIndex_Check(given[i].ptr()) ||
                                 PyNumber_Check(given[i].ptr()),

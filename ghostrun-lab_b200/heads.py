@@ -10,12 +10,13 @@ tables [choices of part j, choices of part k] for k = 1..4, j < k (policy.Policy
 RlEnv.masks; u: fp32 random numbers in [0, 1), [B, 5] (sample: [B]); ids: int16 packed moves, as RlEnv.actions. sample's
 legal is [B, V], or the 19 mask bytes for a flat head over the 324 packed moves, or None.
 
-temperature (0: the best choice), top_k (0: all), top_p and min_p are numbers, or tensors with one for each row. They apply
-in this order: top-k of the logits / temperature, the shortest run of what is left that holds top_p of its probability,
-those of it with at least min_p of the best one's. Equal logits rank by index. The log-probability returned is that of the
-distribution drawn from. The same inputs give the same choice on any launch shape (csrc/heads.cuh). The samplers'
-log-probabilities carry no gradient: moves_logp gives the moves' own. A part (or row) with nothing legal answers 0, the neutral
-choice, with log-probability and entropy 0 and no gradient."""
+temperature (0: the best choice), top_k (0: all), top_p and min_p are numbers, or tensors [B] with one for each row. They
+apply in this order: top-k of the logits / temperature, the shortest run of what is left that holds top_p of its probability,
+those of it with at least min_p of the best one's. Numbers out of range are refused; a row's own count as the nearest that is
+allowed (top_k, top_p and temperature below 0 as 0, min_p above 1 as 1), NaN as a temperature of 0 or as no cut. Equal logits
+rank by index. The log-probability returned is that of the distribution drawn from. The same inputs give the same choice on
+any launch shape (csrc/heads.cuh). The samplers' log-probabilities carry no gradient: moves_logp gives the moves' own. A part
+(or row) with nothing legal answers 0, the neutral choice, with log-probability and entropy 0 and no gradient."""
 from __future__ import annotations
 
 import policy_ops

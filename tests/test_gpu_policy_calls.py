@@ -1,12 +1,12 @@
-"""What the policy operators' calls take and refuse beyond their values: forward-mode derivatives (norm.py, heads.py,
-csrc/policy_ops.cpp)."""
+"""What the policy operators' calls take and refuse beyond their values: forward-mode derivatives, and whole
+numbers of more than 32 bits (norm.py, heads.py, csrc/policy_ops.cpp)."""
 from __future__ import annotations
 
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
 
-from heads import SIZES, TABLES, _lib, moves_logp
+from heads import SIZES, TABLES, _lib, moves_logp, sample, sample_moves
 from norm import layer_norm
 
 
@@ -44,3 +44,18 @@ def test_tangents_are_refused_not_lost(lib, grad):
             with pytest.raises(RuntimeError, match='moves_logp: .*forward-mode'):
                 moves_logp(t[0], t[1:], masks, ids)
     assert layer_norm(x, w, b).shape == x.shape   # without one, as before
+
+
+@pytest.mark.gpu
+def test_top_k_of_each_row_in_64_bits(lib):
+    """A whole number past 31 bits is as large as it says: more than any row has, not what its low bits are."""
+    g = torch.Generator(device='cuda').manual_seed(3)
+    l = torch.randn(8, 50, generator=g, device='cuda')
+    u = torch.rand(8, generator=g, device='cuda')
+    k = torch.tensor([2 ** 32 + 1, 2 ** 32 + 5, 2 ** 31, 2 ** 33, 2 ** 63 - 1, -2 ** 32 + 1, -2 ** 63, 3], device='cuda')
+    want = torch.tensor([50, 50, 50, 50, 50, 0, 0, 3], dtype=torch.int32, device='cuda')   # below 0: all, as 0
+    assert all(torch.equal(a, b) for a, b in zip(sample(l, u, top_k=k), sample(l, u, top_k=want)))
+    logits, cond, masks, _ = _heads(8, 4)
+    v = torch.rand(8, 5, generator=g, device='cuda')
+    got, ref = (sample_moves(logits, cond, masks, v, top_k=n) for n in (k, want))
+    assert all(torch.equal(a, b) for a, b in zip(got, ref))

@@ -440,6 +440,7 @@ py::tuple moves_logp(const Tensor& logits_, const std::optional<std::vector<Tens
 }  // namespace
 
 PYBIND11_MODULE(policy_ops_b200, m) {
+    m.attr("built_for") = BUILT_FOR;   // build.py looks for it in the file
     m.def("bind", &bind);
     m.def("layer_norm", &layer_norm);
     m.def("sample_moves", &sample_moves);

@@ -8,8 +8,10 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <atomic>
 #include <cmath>
 #include <limits>
+#include <memory>
 #include <optional>
 #include <string>
 #include <vector>
@@ -34,7 +36,17 @@ struct Library {
     decltype(&rl_moves_logp_bwd_work_bytes) moves_logp_bwd_work_bytes = nullptr;
     decltype(&rl_moves_logp_bwd) moves_logp_bwd = nullptr;
     decltype(&rl_heads_error) heads_error = nullptr;
-} lib;
+};
+
+// The functions that calls use: all ten at once, since a backward may run while another library is bound. An older table
+// stays, a call may be in it.
+std::atomic<const Library*> bound{nullptr};
+
+const Library& library() {
+    const Library* lib = bound.load(std::memory_order_acquire);
+    TORCH_CHECK(lib, "policy_ops_b200 has no library yet: policy_ops.load() gives it one");
+    return *lib;
+}
 
 template <class F>
 void take(const py::dict& addresses, const char* name, F& f) {
@@ -42,16 +54,18 @@ void take(const py::dict& addresses, const char* name, F& f) {
 }
 
 void bind(const py::dict& at) {
-    take(at, "rl_norm_fwd", lib.norm_fwd);
-    take(at, "rl_norm_bwd_work_bytes", lib.norm_bwd_work_bytes);
-    take(at, "rl_norm_bwd", lib.norm_bwd);
-    take(at, "rl_norm_error", lib.norm_error);
-    take(at, "rl_moves_sample", lib.moves_sample);
-    take(at, "rl_sample", lib.sample);
-    take(at, "rl_moves_logp", lib.moves_logp);
-    take(at, "rl_moves_logp_bwd_work_bytes", lib.moves_logp_bwd_work_bytes);
-    take(at, "rl_moves_logp_bwd", lib.moves_logp_bwd);
-    take(at, "rl_heads_error", lib.heads_error);
+    auto lib = std::make_unique<Library>();
+    take(at, "rl_norm_fwd", lib->norm_fwd);
+    take(at, "rl_norm_bwd_work_bytes", lib->norm_bwd_work_bytes);
+    take(at, "rl_norm_bwd", lib->norm_bwd);
+    take(at, "rl_norm_error", lib->norm_error);
+    take(at, "rl_moves_sample", lib->moves_sample);
+    take(at, "rl_sample", lib->sample);
+    take(at, "rl_moves_logp", lib->moves_logp);
+    take(at, "rl_moves_logp_bwd_work_bytes", lib->moves_logp_bwd_work_bytes);
+    take(at, "rl_moves_logp_bwd", lib->moves_logp_bwd);
+    take(at, "rl_heads_error", lib->heads_error);
+    bound.store(lib.release(), std::memory_order_release);
 }
 
 // The library's number of a type; -1: none of its three.
@@ -110,6 +124,7 @@ struct Normed {
 
 Normed norm_forward(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, double eps, const MaybeTensor& residual,
                     at::ScalarType out_type, bool want_stats) {
+    const Library& lib = library();
     const int64_t width = x.size(-1);
     const Tensor x2 = rows_of(x, width), r2 = residual ? rows_of(*residual, width) : Tensor();
     const MaybeTensor w = weight ? MaybeTensor(weight->contiguous()) : std::nullopt;
@@ -143,6 +158,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const Library& lib = library();
         const auto saved = ctx->get_saved_variables();
         const Tensor &s = saved[0], &stats = saved[1], &weight = saved[2];
         const auto shape = ctx->saved_data["shape"].toIntVector();
@@ -316,6 +332,7 @@ struct Cut {
 py::tuple sample_moves(const Tensor& logits_, const std::optional<std::vector<Tensor>>& cond_, const Tensor& masks_, const Tensor& u_,
                        const py::object& temperature, const py::object& top_k, const py::object& top_p, const py::object& min_p) {
     const char* what = "sample_moves";
+    const Library& lib = library();
     const Tensor logits = check_logits(what, logits_, kBytes);
     const c10::cuda::CUDAGuard guard(logits.device());
     const int64_t rows = logits.size(0);
@@ -336,6 +353,7 @@ py::tuple sample_moves(const Tensor& logits_, const std::optional<std::vector<Te
 py::tuple sample(const Tensor& logits_, const Tensor& u_, const MaybeTensor& legal_, const py::object& temperature,
                  const py::object& top_k, const py::object& top_p, const py::object& min_p) {
     const char* what = "sample";
+    const Library& lib = library();
     const Tensor logits = check_logits(what, logits_, 0);
     const c10::cuda::CUDAGuard guard(logits.device());
     const int64_t rows = logits.size(0), width = logits.size(1);
@@ -354,6 +372,7 @@ py::tuple sample(const Tensor& logits_, const Tensor& u_, const MaybeTensor& leg
 }
 
 variable_list logp_forward(const Tensor& logits, const Tensor& masks, const Tensor& ids, at::TensorList cond) {
+    const Library& lib = library();
     const int64_t rows = logits.size(0);
     const Tensor logp = make({rows}, at::kFloat, logits), entropy = make({rows}, at::kFloat, logits);
     const Tables tables(cond);
@@ -378,6 +397,7 @@ struct MovesLogp : torch::autograd::Function<MovesLogp> {
     }
 
     static variable_list gradients(AutogradContext* ctx, variable_list grads) {
+        const Library& lib = library();
         const auto saved = ctx->get_saved_variables();
         const Tensor &logits = saved[0], &masks = saved[1], &ids = saved[2];
         const at::ArrayRef<Tensor> cond = at::ArrayRef<Tensor>(saved).slice(3);

@@ -15,7 +15,8 @@ _LIB = None
 
 
 def load(path=None):
-    """The library, with the C-ABI's argument types, bound to policy_ops_b200; another path takes the place of the one before."""
+    """The library, with the C-ABI's argument types, bound to policy_ops_b200; another path takes the place of the one
+    before, for every later call in the process."""
     global _LIB
     if _LIB is None or path is not None:
         try:

@@ -1,5 +1,5 @@
-"""What the policy operators' calls take and refuse beyond their values: forward-mode derivatives, and whole
-numbers of more than 32 bits (norm.py, heads.py, csrc/policy_ops.cpp)."""
+"""What the policy operators' calls take and refuse beyond their values: forward-mode derivatives, whole numbers of
+more than 32 bits, and CUDA graphs that hold both directions (norm.py, heads.py, csrc/policy_ops.cpp)."""
 from __future__ import annotations
 
 import pytest
@@ -59,3 +59,38 @@ def test_top_k_of_each_row_in_64_bits(lib):
     v = torch.rand(8, 5, generator=g, device='cuda')
     got, ref = (sample_moves(logits, cond, masks, v, top_k=n) for n in (k, want))
     assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
+@pytest.mark.gpu
+def test_both_directions_in_a_graph(lib):
+    """A captured step of the norm and the log-probabilities with their gradients, played again on new inputs: the bits of the
+    same step outside the graph."""
+    g = torch.Generator(device='cuda').manual_seed(5)
+    x = torch.randn(600, 512, generator=g, device='cuda').bfloat16().requires_grad_(True)
+    r = torch.randn(600, 512, generator=g, device='cuda').bfloat16().requires_grad_(True)
+    w, b = (torch.randn(512, generator=g, device='cuda').requires_grad_(True) for _ in range(2))
+    gy, gs = (torch.randn(600, 512, generator=g, device='cuda').bfloat16() for _ in range(2))
+    logits, cond, masks, ids = _heads(600, 6)
+    leaves = [t.requires_grad_(True) for t in (logits, *cond)]
+    ga = torch.randn(600, generator=g, device='cuda')
+
+    def step():
+        out = layer_norm(x, w, b, residual=r)
+        lp = moves_logp(leaves[0], leaves[1:], masks, ids)
+        return [t.detach() for t in (*out, *lp)] + [*torch.autograd.grad(out, (x, w, b, r), (gy, gs)),
+                                                    *torch.autograd.grad(lp, leaves, (ga, ga))]
+
+    q = torch.cuda.Stream()
+    q.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(q):
+        step()
+    torch.cuda.current_stream().wait_stream(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    with torch.no_grad():
+        for t in (x, r, w, b, gy, logits):
+            t.mul_(0.75)
+    graph.replay()
+    want = step()
+    assert all(torch.equal(a, c) for a, c in zip(held, want))

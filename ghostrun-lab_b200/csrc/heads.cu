@@ -11,9 +11,9 @@
 // A part with nothing legal answers its choice 0 (neutral, off), and adds 0 to the log-probability, the entropy and the
 // gradients. Masked logits are never used, whatever they hold.
 //
-// A row is 19 logits and some 50 bytes more, and some 900 (a draw), 700 (log-probabilities) or 900 (gradients) instructions: on
-// 8,192 x 128 rows the kernels issue in 80 %, 75 % and 50 % of their cycles, and take 37, 33 and 59 us where the bytes alone
-// would take 13, 17 and 29.
+// A row is 19 logits and some 50 bytes more, and some 970 (a draw), 780 (log-probabilities) or 920 (gradients) instructions: on
+// 8,192 x 128 rows the kernels issue in 81 %, 76 % and 50 % of their cycles, and take 37, 34 and 60 us where the bytes alone
+// would take 13, 17 and 29. A draw with every truncation takes 66 us there: the ranks and the sums before each choice.
 #include "heads.cuh"
 
 using namespace heads;
@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(kThreads) k_moves_logp(LogpArgs a) {
 // order of the additions is the launch's alone; the 23 additions of a row go to 23 places, so they are read together and
 // written together. The columns' 508 bytes per thread leave 8 to 10 warps per SM, so a thread takes R = 2 rows side by side
 // where there are rows for it (8,192 x 128 rows: 76 us with one row per thread and the next batch on its way, 80 us with two
-// and 256 threads, 70 us with two and 128, 59 us with two and blocks of 64); one row each where every block has one batch
+// and 256 threads, 70 us with two and 128, 60 us with two and blocks of 64); one row each where every block has one batch
 // at most.
 template <class T, int THREADS, int R>
 __global__ void __launch_bounds__(THREADS) k_moves_grad(LogpArgs a) {

@@ -1,7 +1,7 @@
 // One choice for each row of logits, 1 to 4,096 wide (a flat head over the 324 packed moves, legal under the same 19 mask bytes,
 // for one), with temperature, top-k, top-p and min-p; the definition of a draw stands in heads.cuh. What a row costs is its
-// instructions, not its bytes (8,192 rows of 324 bf16 read 5.6 MB, 0.9 us, and take 9 us with no truncation, most of it exp and
-// the sums, and 19 us with top-p): a row stays in a warp's registers (in a block's from 1,025 choices on), and a truncation
+// instructions, not its bytes (8,192 rows of 324 bf16 read 5.6 MB, 0.9 us, and take 10 us with no truncation, most of it exp and
+// the sums, and 17 us with top-p): a row stays in a warp's registers (in a block's from 1,025 choices on), and a truncation
 // is found without sorting.
 #include "heads.cuh"
 
@@ -93,11 +93,6 @@ struct Team {
         join<false, false>(a, b);
         total = a & ((1ull << 44) - 1);
         count = static_cast<unsigned>(a >> 44);
-    }
-    __device__ u64 sum(u64 v) {
-        u64 a = warp_total(v), b = 0;
-        join<false, false>(a, b);
-        return a;
     }
     __device__ unsigned count(unsigned n) {
         u64 a = __reduce_add_sync(~0u, n), b = 0;
@@ -549,8 +544,9 @@ k_rows_sample(RowArgs a) {
             const unsigned k = static_cast<unsigned>(q.top_k);
             if (k < kept) cut_row<false>(r, team, few, k, m, -INFINITY, kth_bound(r, team, k), kept);
         }
-        // what a small k left of a wide row is one warp's work (2,049 x 4,001 with every truncation: 64 us without, 56 with it;
-        // without a top-p to follow it does not pay, 34 us against 40)
+        // what a small k left of a wide row is one warp's work (2,049 rows, top-p 0.9, without and with it: at top-k 50 31 and 28 us
+        // for 1,500 choices, 59 and 53 for 2,049, 70 and 64 for 4,001; at top-k 128 31 and 29 for 1,025, 74 and 66 for 4,001; at
+        // top-k 2 23.9 and 24.2 for 1,025, 57 and 55 for 4,001; without a top-p to follow it does not pay)
         if constexpr (TPR > 32) {
             if (q.top_p < 1.f && q.top_k > 0 && q.top_k <= kFew && kept > static_cast<unsigned>(q.top_k)) {
                 gather(r, team, few_s[0]);
@@ -623,7 +619,7 @@ int rl_sample(const void* logits, long long stride, int type, int width, const v
     with_type(type, [&](auto t) {
         using T = decltype(t);
         with_row_tile(width, [&](auto tpr, auto ept) {
-            // more blocks than fit at once: the last ones even out (8,192 x 324: 18.0 us with as many as fit, 16.6 with twice that)
+            // more blocks than fit at once: the last ones even out (8,192 x 324: 1.4 us less than with as many as fit)
             const unsigned grid = tpr() == 32 ? blocks_for(rows, 8, 2 * kRowWarps<ept()> / 8ll * sm_count())
                                               : blocks_for(rows, 1, 16 * kRowWarps<ept()> * 32ll / tpr() * sm_count());
             const unsigned block = tpr() == 32 ? 256 : tpr();

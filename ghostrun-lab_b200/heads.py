@@ -50,5 +50,6 @@ def sample(logits, u, legal=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
 def moves_logp(logits, cond, masks, ids, lib_path=None):
     """(log-probability, entropy) fp32 [B] of the moves ids under the ordered heads, the entropy the sum of the parts'
     conditional entropies along the move. A move that the masks exclude has log-probability -inf, an id outside 0..323 NaN
-    in both."""
+    in both. The backward reads logits, cond, masks and ids again: give it copies of buffers that the env writes
+    (RlEnv.masks, RlEnv.actions) where a step may come between."""
     return _ready(lib_path).moves_logp(logits, cond, masks, ids)
